@@ -318,6 +318,71 @@ int gmk_fid_from_moments(const double* G1, const double* s1, int64_t n1, const d
 int gmk_softmax_stats(const float* logits, int64_t n, int C, int topn, float eps, double* out,
                       gmk_stream_t stream);
 
+/* ---------------------------------------------------------------- a classifier made smaller ----------
+ * Teacher to student, no counterpart in the reference (its classifier is trained on labels and answers in fp32,
+ * models/classifiers.py:77-113): the teacher's fully connected layers answer in 8-bit integers (gmk_linear_i8_fwd), the k
+ * largest logits of every sample are kept (gmk_topk_rows), and the student learns from them (gmk_distill_*).
+ * Floating tensors are fp32, bf16 or fp16 (gmk_dtype), row-major and contiguous, aligned to their element; every sum, maximum and
+ * scale is held in 32 bits or more, and values are rounded to the output's type once.  Calls with zero rows launch nothing and
+ * return 0.  8-bit buffers and workspaces are 16-byte aligned; outputs overlap no input.  Results do not depend on the launch's
+ * timing (no float atomics). */
+enum gmk_dtype { GMK_F32 = 0, GMK_BF16 = 1, GMK_F16 = 2 };
+
+/* gmk_quantize_rows: x (M,K) -> q (M,ldq) int8, scale (M) fp32, one scale for each row:
+ *   scale = max(fl32(max_k |x| / 127), 2^-126), q = the whole number nearest x / scale (halves to even; exact, whatever the
+ *   quotient's own rounding), zeros in columns [K, ldq).  ldq >= K, ldq % 16 == 0.  A row that holds an infinity or a NaN
+ *   gets zeros and a NaN scale, so that whatever is made of it is NaN. */
+int gmk_quantize_rows(const void* x, int xtype, signed char* q, float* scale, int64_t M, int K, int ldq,
+                      gmk_stream_t stream);
+
+/* gmk_gemm_i8: y (M,N) = act((sum_k xq[m][k] wq[n][k]) * xscale[m] * wscale[n] + bias[n]), the sum exact in 32-bit
+ *   integers.  xq (M,K), wq (N,K) int8 in [-128, 127], K % 16 == 0 (rows that gmk_quantize_rows padded are whole), K <= GMK_I8_MAX_K;
+ *   bias (N) fp32 or NULL; act: enum gmk_act.  ws >= gmk_gemm_i8_workspace_bytes(M, K, N) bytes. */
+#define GMK_I8_MAX_K 131056
+size_t gmk_gemm_i8_workspace_bytes(int M, int K, int N);
+int gmk_gemm_i8(const signed char* xq, const float* xscale, const signed char* wq, const float* wscale, const float* bias,
+                void* y, int ytype, int M, int K, int N, int act, void* ws, size_t ws_bytes, gmk_stream_t stream);
+/* gmk_linear_i8_fwd: the same from floating activations: x (M,K) is quantised row by row as gmk_quantize_rows does, and
+ *   wq (N, ldw) holds the weight's rows as gmk_quantize_rows wrote them once, ldw = K rounded up to 16.  K <= GMK_I8_MAX_K.
+ *   The 8-bit counterpart of gmk_linear_fwd, for inference (no derivative).  ws >= gmk_linear_i8_workspace_bytes(M, K, N). */
+size_t gmk_linear_i8_workspace_bytes(int M, int K, int N);
+int gmk_linear_i8_fwd(const void* x, int xtype, const signed char* wq, const float* wscale, const float* bias, void* y,
+                      int ytype, int M, int K, int N, int act, void* ws, size_t ws_bytes, gmk_stream_t stream);
+
+/* gmk_topk_rows: the k largest of each row of x (n,C): value (n,k) in x's type, index (n,k) int32, in falling order, equal
+ *   values by rising index.  -0 equals 0; a NaN ranks above every number; masked classes (-inf, the type's lowest) are ordinary
+ *   values.  1 <= k <= min(C, GMK_TOPK_MAX), C < 2^31.  ws >= gmk_topk_rows_workspace_bytes(n, C, k) bytes (0: NULL is fine). */
+#define GMK_TOPK_MAX 256
+size_t gmk_topk_rows_workspace_bytes(int64_t n, int64_t C, int k);
+int gmk_topk_rows(const void* x, int xtype, void* value, int* index, int64_t n, int64_t C, int k, void* ws, size_t ws_bytes,
+                  gmk_stream_t stream);
+
+/* gmk_distill_*: the loss of a student's logits z (n,C) against a teacher's kept logits t (n,k) of the classes idx (n,k), and
+ *   against labels:
+ *     q = softmax(z / T) over all C classes, p = softmax(t / T) over the row's entries, p_c = sum_{j: idx_j = c} p_j,
+ *     loss = soft T^2 sum_j p_j (ln p_j - ln q_{idx_j}) + hard (-ln softmax(z)_label),
+ *     d loss / d z_c = soft T (q_c - p_c) + hard (softmax(z)_c - [c = label]).
+ *   An idx outside [0, C) is no entry, and a row without an entry of a weight above 0 has no soft part; a label outside [0, C)
+ *   (say -100) or labels == NULL: no hard part.  A row whose logits are all -inf gives loss 0 and gradient 0.  The same class may be
+ *   listed more than once.  z and dz share ztype, t has ttype.  1 <= k <= GMK_DISTILL_MAX_K, C < 2^31, T > 0.
+ * gmk_distill_fwd: loss (n) fp32 and stats (n,3) fp32 (the row's maximum and its two sums of exponentials) for the backward pass.
+ * gmk_distill_bwd: dz (n,C) = grad[row] * d loss / d z, grad (n) fp32.  Rows with grad 0 give 0 (nothing of them is read).
+ * gmk_distill_fwd_bwd: both in one call, each logit read from memory once where a row fits the registers of a workgroup:
+ *   loss[row] = weight[row] * loss, dz = scale * weight[row] * d loss / d z; weight (n) fp32, or NULL for ones.  Rows with
+ *   weight 0 (padding) give 0 and 0 whatever they hold.
+ *   ws >= gmk_distill_workspace_bytes(n, C) bytes (0: NULL is fine), the same for all three. */
+#define GMK_DISTILL_MAX_K 256
+size_t gmk_distill_workspace_bytes(int64_t n, int64_t C);
+int gmk_distill_fwd(const void* z, int ztype, const void* t, int ttype, const int* idx, const int64_t* labels, float* loss,
+                    float* stats, int64_t n, int64_t C, int k, float T, float soft, float hard, void* ws, size_t ws_bytes,
+                    gmk_stream_t stream);
+int gmk_distill_bwd(const float* grad, const void* z, int ztype, const void* t, int ttype, const int* idx,
+                    const int64_t* labels, const float* stats, void* dz, int64_t n, int64_t C, int k, float T, float soft,
+                    float hard, gmk_stream_t stream);
+int gmk_distill_fwd_bwd(const void* z, int ztype, const void* t, int ttype, const int* idx, const int64_t* labels,
+                        const float* weight, float* loss, void* dz, int64_t n, int64_t C, int k, float T, float soft,
+                        float hard, float scale, void* ws, size_t ws_bytes, gmk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
