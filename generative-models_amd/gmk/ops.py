@@ -3,6 +3,7 @@
 Every function takes contiguous fp32 CUDA tensors, allocates its outputs with torch (device
 memory plumbing), and launches on torch's current stream.
 """
+import functools
 import os
 import torch
 
@@ -544,128 +545,140 @@ def softmax_stats(logits, out=None, topn=3, eps=1e-7):
 # These take fp32, bf16 or fp16 tensors.  Their scratch is a tensor of the call's own, from torch's allocator: calls on different
 # streams and captured graphs share none of it.
 _FLOAT_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FP32, _INT8, _INT32, _INT64 = (torch.float32,), (torch.int8,), (torch.int32,), (torch.int64,)
 I8_MAX_K, TOPK_MAX, DISTILL_MAX_K = 131056, 256, 256   # include/gmk.h
 
 
-def _chk_rows(name, t, dtypes, shape, device):
-    """`t` is a contiguous CUDA tensor of one of `dtypes`, on `device`, its shape `shape` (None: any size)."""
+def _chk_rows(name, t, dtypes, shape, dev):
+    """`t` is a contiguous tensor on GPU number `dev`, of one of `dtypes` and of this shape (None: of any two sizes)."""
+    if (isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype in dtypes and t.is_contiguous() and
+            (t.shape == shape or (shape is None and t.dim() == 2))):
+        return
     if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous() or t.dtype not in dtypes:
         raise ValueError(f"{name} must be a contiguous CUDA tensor of type {' or '.join(str(d) for d in dtypes)}")
-    if t.dim() != len(shape) or any(want is not None and have != want for have, want in zip(t.shape, shape)):
-        raise ValueError(f"{name} must have the shape {tuple('any' if s is None else s for s in shape)}, not {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the first argument on {device}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the first argument on cuda:{dev}")
+    raise ValueError(f"{name} must have {'two dimensions' if shape is None else f'the shape {tuple(shape)}'}, not the shape {tuple(t.shape)}")
 
 
-def _chk_device(x):
-    """A launch goes to the current device's stream: tensors of another device are refused."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+def _chk_first(name, t, dtypes):
+    """The number of the GPU that a call's first tensor (n, C) is on.  It has to be the current one, whose stream the launch goes
+    to.  (torch._C's getters: torch.cuda's cost the smallest calls several microseconds.)"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("gmk ops need CUDA tensors")
-    if x.device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+    dev = t.get_device()
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    _chk_rows(name, t, dtypes, None, dev)
+    return dev
 
 
-def _scratch(nbytes, device):
-    return _new(int(nbytes), device, torch.uint8) if nbytes else None
+def _stream_of(dev):
+    return _cur_stream if _cur_stream is not None else torch._C._cuda_getCurrentRawStream(dev)
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(name, *sizes):
+    return int(getattr(lib(), name)(*sizes))
+
+
+def _scratch(device, name, *sizes):
+    """(tensor or None, its bytes) of the scratch that an entry point asks for."""
+    nbytes = _scratch_bytes(name, *sizes)
+    return (_new(nbytes, device, torch.uint8), nbytes) if nbytes else (None, 0)
 
 
 def quantize_rows(x):
     """x (M, K) -> (q (M, K rounded up to 16) int8, scale (M,) fp32): each row in 8 bits, x ~ q * scale, zeros behind column K.
     Weights (rows = output channels) are quantised by it once, activations by linear_i8 in every call."""
-    _chk_device(x)
-    _chk_rows("x", x, tuple(_FLOAT_IDS), (None, None), x.device)
+    dev = _chk_first("x", x, _FLOAT_IDS)
     M, K = x.shape
     if K == 0:
         raise ValueError("x must have at least one column")
     ld = -(-K // 16) * 16
     q = _new((M, ld), x.device, torch.int8)
     scale = _new((M,), x.device, torch.float32)
-    check(lib().gmk_quantize_rows(_p(x), _FLOAT_IDS[x.dtype], _p(q), _p(scale), M, K, ld, _stream()))
+    check(lib().gmk_quantize_rows(_p(x), _FLOAT_IDS[x.dtype], _p(q), _p(scale), M, K, ld, _stream_of(dev)))
     return q, scale
 
 
-def _i8_args(x, K, wq, wscale, bias, out_dtype):
+def _i8_args(dev, K, wq, wscale, bias, out_dtype):
     if out_dtype not in _FLOAT_IDS:
         raise ValueError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
     if K == 0 or K > I8_MAX_K:
         raise ValueError(f"the 8-bit product takes 1 to {I8_MAX_K} columns, not {K}")
-    _chk_rows("wq", wq, (torch.int8,), (None, -(-K // 16) * 16), x.device)
-    N = wq.shape[0]
-    if N == 0:
-        raise ValueError("wq must have at least one row")
-    _chk_rows("wscale", wscale, (torch.float32,), (N,), x.device)
+    _chk_rows("wq", wq, _INT8, None, dev)
+    N, ld = wq.shape
+    if N == 0 or ld != -(-K // 16) * 16:
+        raise ValueError(f"wq must have at least one row and {-(-K // 16) * 16} columns ({K} rounded up to 16), not {tuple(wq.shape)}")
+    _chk_rows("wscale", wscale, _FP32, (N,), dev)
     if bias is not None:
-        _chk_rows("bias", bias, (torch.float32,), (N,), x.device)
+        _chk_rows("bias", bias, _FP32, (N,), dev)
     return N
 
 
 def matmul_i8(xq, xscale, wq, wscale, bias=None, act=None, out_dtype=torch.float32):
     """act((xq @ wq.T) * xscale[:, None] * wscale + bias) for rows that quantize_rows made; the sum is exact."""
-    _chk_device(xq)
-    _chk_rows("xq", xq, (torch.int8,), (None, None), xq.device)
+    dev = _chk_first("xq", xq, _INT8)
     M, K = xq.shape
     if K % 16:
         raise ValueError(f"xq has {K} columns: rows of 8-bit values are padded to a multiple of 16 (quantize_rows)")
-    _chk_rows("xscale", xscale, (torch.float32,), (M,), xq.device)
-    N = _i8_args(xq, K, wq, wscale, bias, out_dtype)
+    _chk_rows("xscale", xscale, _FP32, (M,), dev)
+    N = _i8_args(dev, K, wq, wscale, bias, out_dtype)
     y = _new((M, N), xq.device, out_dtype)
-    ws = _scratch(lib().gmk_gemm_i8_workspace_bytes(M, K, N), xq.device)
+    ws, nbytes = _scratch(xq.device, "gmk_gemm_i8_workspace_bytes", M, K, N)
     check(lib().gmk_gemm_i8(_p(xq), _p(xscale), _p(wq), _p(wscale), _p(bias), _p(y), _FLOAT_IDS[out_dtype], M, K, N, act_id(act),
-                            _p(ws), 0 if ws is None else ws.numel(), _stream()))
+                            _p(ws), nbytes, _stream_of(dev)))
     return y
 
 
 def linear_i8(x, wq, wscale, bias=None, act=None, out_dtype=None):
     """The 8-bit form of linear_fwd for inference: x (M, K) is quantised row by row, the weight's rows are quantize_rows' (q, scale).
     Returns (M, N) in out_dtype (default: x's type)."""
-    _chk_device(x)
-    _chk_rows("x", x, tuple(_FLOAT_IDS), (None, None), x.device)
+    dev = _chk_first("x", x, _FLOAT_IDS)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     M, K = x.shape
-    N = _i8_args(x, K, wq, wscale, bias, out_dtype)
+    N = _i8_args(dev, K, wq, wscale, bias, out_dtype)
     y = _new((M, N), x.device, out_dtype)
-    ws = _scratch(lib().gmk_linear_i8_workspace_bytes(M, K, N), x.device)
+    ws, nbytes = _scratch(x.device, "gmk_linear_i8_workspace_bytes", M, K, N)
     check(lib().gmk_linear_i8_fwd(_p(x), _FLOAT_IDS[x.dtype], _p(wq), _p(wscale), _p(bias), _p(y), _FLOAT_IDS[out_dtype], M, K, N,
-                                  act_id(act), _p(ws), 0 if ws is None else ws.numel(), _stream()))
+                                  act_id(act), _p(ws), nbytes, _stream_of(dev)))
     return y
 
 
 def topk_rows(x, k):
     """The k largest of each row of x (n, C): (values (n, k) of x's type, index (n, k) int32), falling; equal values by rising
     index, NaN above every number."""
-    _chk_device(x)
-    _chk_rows("x", x, tuple(_FLOAT_IDS), (None, None), x.device)
+    dev = _chk_first("x", x, _FLOAT_IDS)
     n, C = x.shape
     k = int(k)
     if not 1 <= k <= min(C, TOPK_MAX):
         raise ValueError(f"k must be between 1 and min({C} columns, {TOPK_MAX}), not {k}")
     value = _new((n, k), x.device, x.dtype)
     index = _new((n, k), x.device, torch.int32)
-    ws = _scratch(lib().gmk_topk_rows_workspace_bytes(n, C, k), x.device)
-    check(lib().gmk_topk_rows(_p(x), _FLOAT_IDS[x.dtype], _p(value), _p(index), n, C, k, _p(ws), 0 if ws is None else ws.numel(),
-                              _stream()))
+    ws, nbytes = _scratch(x.device, "gmk_topk_rows_workspace_bytes", n, C, k)
+    check(lib().gmk_topk_rows(_p(x), _FLOAT_IDS[x.dtype], _p(value), _p(index), n, C, k, _p(ws), nbytes, _stream_of(dev)))
     return value, index
 
 
 def _distill_args(logits, teacher, index, labels, T, soft, hard):
-    """(n, C, k) after the checks that the distillation calls share."""
-    _chk_device(logits)
-    _chk_rows("logits", logits, tuple(_FLOAT_IDS), (None, None), logits.device)
+    """(n, C, k, GPU number) after the checks that the distillation calls share."""
+    dev = _chk_first("logits", logits, _FLOAT_IDS)
     n, C = logits.shape
     if C == 0:
         raise ValueError("logits must have at least one class")
-    _chk_rows("teacher", teacher, tuple(_FLOAT_IDS), (n, None), logits.device)
+    _chk_rows("teacher", teacher, _FLOAT_IDS, None, dev)
     k = teacher.shape[1]
-    if not 1 <= k <= DISTILL_MAX_K:
-        raise ValueError(f"teacher must hold 1 to {DISTILL_MAX_K} logits a row, not {k}")
-    _chk_rows("index", index, (torch.int32,), (n, k), logits.device)
+    if teacher.shape[0] != n or not 1 <= k <= DISTILL_MAX_K:
+        raise ValueError(f"teacher must hold 1 to {DISTILL_MAX_K} logits for each of {n} rows, not {tuple(teacher.shape)}")
+    _chk_rows("index", index, _INT32, (n, k), dev)
     if labels is not None:
-        _chk_rows("labels", labels, (torch.int64,), (n,), logits.device)
+        _chk_rows("labels", labels, _INT64, (n,), dev)
     elif hard != 0:
         raise ValueError("a hard part needs labels")
     if not 0 < T < float("inf") or soft - soft != 0 or hard - hard != 0:
         raise ValueError("the temperature must be finite and above 0, the weights finite")
-    return n, C, k
+    return n, C, k, dev
 
 
 def distill_fwd(logits, teacher, index, labels=None, T=1.0, soft=1.0, hard=0.0):
@@ -673,37 +686,37 @@ def distill_fwd(logits, teacher, index, labels=None, T=1.0, soft=1.0, hard=0.0):
     (a class outside [0, C): no entry) and against labels (n,) int64 (outside [0, C): none):
     soft T^2 KL(softmax(teacher / T) || softmax(logits / T)) + hard CE(logits, labels).  Returns (loss (n,), stats (n, 3)), stats
     for distill_bwd."""
-    n, C, k = _distill_args(logits, teacher, index, labels, T, soft, hard)
+    n, C, k, dev = _distill_args(logits, teacher, index, labels, T, soft, hard)
     loss = _new((n,), logits.device, torch.float32)
     stats = _new((n, 3), logits.device, torch.float32)
-    ws = _scratch(lib().gmk_distill_workspace_bytes(n, C), logits.device)
+    ws, nbytes = _scratch(logits.device, "gmk_distill_workspace_bytes", n, C)
     check(lib().gmk_distill_fwd(_p(logits), _FLOAT_IDS[logits.dtype], _p(teacher), _FLOAT_IDS[teacher.dtype], _p(index), _p(labels),
                                 _p(loss), _p(stats), n, C, k, float(T), float(soft), float(hard), _p(ws),
-                                0 if ws is None else ws.numel(), _stream()))
+                                nbytes, _stream_of(dev)))
     return loss, stats
 
 
 def distill_bwd(grad, logits, teacher, index, labels, stats, T=1.0, soft=1.0, hard=0.0):
     """grad (n,) fp32, the gradient of each row's loss -> the gradient of the logits, in their type."""
-    n, C, k = _distill_args(logits, teacher, index, labels, T, soft, hard)
-    _chk_rows("grad", grad, (torch.float32,), (n,), logits.device)
-    _chk_rows("stats", stats, (torch.float32,), (n, 3), logits.device)
+    n, C, k, dev = _distill_args(logits, teacher, index, labels, T, soft, hard)
+    _chk_rows("grad", grad, _FP32, (n,), dev)
+    _chk_rows("stats", stats, _FP32, (n, 3), dev)
     dz = _new_like(logits)
     check(lib().gmk_distill_bwd(_p(grad), _p(logits), _FLOAT_IDS[logits.dtype], _p(teacher), _FLOAT_IDS[teacher.dtype], _p(index),
-                                _p(labels), _p(stats), _p(dz), n, C, k, float(T), float(soft), float(hard), _stream()))
+                                _p(labels), _p(stats), _p(dz), n, C, k, float(T), float(soft), float(hard), _stream_of(dev)))
     return dz
 
 
 def distill_fwd_bwd(logits, teacher, index, labels=None, T=1.0, soft=1.0, hard=0.0, weight=None, scale=1.0):
     """Loss and gradient in one call, for a training loop without autograd: (weight * loss (n,), d(scale * sum(weight * loss)) /
     d logits).  weight (n,) fp32 or None; a row of weight 0 (padding) gives zeros whatever it holds."""
-    n, C, k = _distill_args(logits, teacher, index, labels, T, soft, hard)
+    n, C, k, dev = _distill_args(logits, teacher, index, labels, T, soft, hard)
     if weight is not None:
-        _chk_rows("weight", weight, (torch.float32,), (n,), logits.device)
+        _chk_rows("weight", weight, _FP32, (n,), dev)
     loss = _new((n,), logits.device, torch.float32)
     dz = _new_like(logits)
-    ws = _scratch(lib().gmk_distill_workspace_bytes(n, C), logits.device)
+    ws, nbytes = _scratch(logits.device, "gmk_distill_workspace_bytes", n, C)
     check(lib().gmk_distill_fwd_bwd(_p(logits), _FLOAT_IDS[logits.dtype], _p(teacher), _FLOAT_IDS[teacher.dtype], _p(index),
                                     _p(labels), _p(weight), _p(loss), _p(dz), n, C, k, float(T), float(soft), float(hard),
-                                    float(scale), _p(ws), 0 if ws is None else ws.numel(), _stream()))
+                                    float(scale), _p(ws), nbytes, _stream_of(dev)))
     return loss, dz

@@ -136,6 +136,31 @@ def test_gemm_i8_whole_numbers(M):
         assert torch.equal(y.cpu().double(), xq.double() @ wq.double().T)
 
 
+# shapes for each of the larger kernels (64x32, 64x64, 128x128 twice, 256x256 with one and with several tiles a workgroup), ended by all
+# three sizes inside a tile; the smaller ones are in SHAPES
+@gpu
+@pytest.mark.parametrize("shape", [(7, 208, 20000), (30, 1040, 17000), (65, 1040, 17010), (1100, 1296, 3101), (777, 1360, 5003), (1500, 1360, 5003), (4090, 2064, 4085),
+                                   (8190, 144, 8190), (8190, 1040, 4099)])
+def test_gemm_i8_larger_kernels(shape):
+    """Whole numbers below 2^24 in fp32 are exact; bias, activation and a 16-bit output against the same in 64 bits."""
+    from gmk import ops
+    M, K, N = shape
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    xq, wq = (torch.randint(-60, 61, (n, K), generator=g, device="cuda").to(torch.int8) for n in (M, N))
+    one = torch.ones(max(M, N), device="cuda")
+    ref = xq.double() @ wq.double().t().contiguous()
+    assert torch.equal(ops.matmul_i8(xq, one[:M].contiguous(), wq, one[:N].contiguous()).double(), ref)
+    xs, ws, b = (torch.rand(n, generator=g, device="cuda") + 0.5 for n in (M, N, N))
+    xs = xs / K
+    for act, dtype in (("relu", torch.bfloat16), ("gelu", torch.float16), ("elu", torch.float32)):
+        y = ops.matmul_i8(xq, xs, wq, ws, b, act=act, out_dtype=dtype).double()
+        z = ref * xs.double()[:, None] * ws.double() + b.double()
+        r = _act(act, z)
+        tol = (z.abs() + 2 * b.double()) * (4 * 2.0 ** -24 * 1.13 + 1.5e-7 + 8 * 2.0 ** -24)   # as in test_linear_i8
+        tol += torch.finfo(dtype).eps / 2 * (r.abs() + tol) + (2.0 ** -25 if dtype == torch.float16 else 0)
+        assert ((y - r).abs() <= tol).all(), act
+
+
 @gpu
 @pytest.mark.parametrize("M", [1, 20, 150])
 def test_linear_i8_rows_are_independent_and_nan_stays_in_its_row(M):
