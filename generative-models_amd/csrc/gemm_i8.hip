@@ -309,73 +309,111 @@ static int gemm_i8_tile_launch(const signed char* xq, const float* xscale, const
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------
-// A workgroup makes NT * 16 columns times MT * 16 rows of y; its waves take turns along K, 64 bytes of each row at a time straight
-// from memory into the instruction's registers, U steps in flight, and their sums meet in LDS.  Rows behind the last one are read
-// from the last one and never stored; behind K the weight's piece is zero.
-template <class T, int MT, int NT, int WAVES, int U>
-__global__ __launch_bounds__(64 * WAVES) void gemm_i8_rows_kernel(const signed char* __restrict__ xq, const float* __restrict__ xscale,
+// A workgroup makes NT * 16 columns times 16 rows of y; its waves take turns along K, 64 bytes of each row at a time straight from
+// memory into the instruction's registers, U steps in flight, and their sums meet in LDS.  Rows behind the last one are read from the
+// last one and never stored; behind K the weight's piece is zero.
+// X is the rows' type: 8-bit values with xscale, or, for at most I8_FUSED_ROWS rows of floating numbers, x itself, which every workgroup
+// then quantises into its LDS while its first weights are on their way: one launch instead of two.
+#define I8_FUSED_ROWS 4
+#define I8_FUSED_BYTES 16384   // of quantised rows in LDS: 1x4096 30.0 us (two launches 32.0), 4x4096 10.2 (11.7), but 3x8192 22.1 (20.0)
+template <class T, class X, int NT, int WAVES, int U>
+__global__ __launch_bounds__(64 * WAVES) void gemm_i8_rows_kernel(const X* __restrict__ x, const float* __restrict__ xscale,
                                                                   const signed char* __restrict__ wq, const float* __restrict__ wscale,
                                                                   const float* __restrict__ bias, T* __restrict__ y, int M, int K, int N,
-                                                                  int act, int tiles_m) {
-  __shared__ i32x4 part[WAVES * NT * MT * 64];
+                                                                  int act, int tiles_m, int Kx) {
+  constexpr bool FUSED = !std::is_same<X, signed char>::value;
+  __shared__ i32x4 part[WAVES * NT * 64];
+  __shared__ float xs_row[I8_FUSED_ROWS];
+  extern __shared__ __attribute__((aligned(16))) signed char xlds[];   // FUSED: M rows of K bytes
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, kq = lane >> 4;
-  const int n0 = (int)(blockIdx.x / (unsigned)tiles_m) * NT * 16, m0 = (int)(blockIdx.x % (unsigned)tiles_m) * MT * 16;
+  const int n0 = (int)(blockIdx.x / (unsigned)tiles_m) * NT * 16, m0 = (int)(blockIdx.x % (unsigned)tiles_m) * 16;
   const signed char* wp[NT];
-  const signed char* xp[MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) wp[i] = wq + (int64_t)min(n0 + 16 * i + r, N - 1) * K + kq * 16;
-#pragma unroll
-  for (int j = 0; j < MT; ++j) xp[j] = xq + (int64_t)min(m0 + 16 * j + r, M - 1) * K + kq * 16;
-  i32x4 acc[NT][MT] = {};
-  const int full = K >> 6, steps = (K + 63) >> 6;
-  int s = wave;
-  i32x4 a[U][NT], b[U][MT];
-  auto multiply = [&]() {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][i], b[u][j], acc[i][j], 0, 0, 0);
+  const signed char* xp;
+  if constexpr (FUSED) xp = xlds + min(r, M - 1) * K + kq * 16;
+  else xp = x + (int64_t)min(m0 + r, M - 1) * K + kq * 16;
+  i32x4 acc[NT] = {};
+  const int steps = (K + 63) >> 6;
+  i32x4 a[U][NT], b[U];
+  auto x_step = [&](int u, int s) {
+    const int k = (s + u * WAVES) * 64;
+    b[u] = *(const i32x4*)(xp + (k + kq * 16 < K ? k : -kq * 16));
   };
-  for (; s + (U - 1) * WAVES < full; s += U * WAVES) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = (s + u * WAVES) * 64;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) a[u][i] = *(const i32x4*)(wp[i] + k);
-#pragma unroll
-      for (int j = 0; j < MT; ++j) b[u][j] = *(const i32x4*)(xp[j] + k);
-    }
-    multiply();
-  }
-  if (s < steps) {   // the last U steps of this wave or fewer, one of which K may end in
+  // this wave's steps s, s + WAVES, ...; behind K zeros of the weight (the address is then the row's first one)
+  auto fetch = [&](int s) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = (s + u * WAVES) * 64;
       const bool in = k + kq * 16 < K;
-      const int at = in ? k : 0;   // column kq * 16 need not exist: its row starts at column 0
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const i32x4 v = *(const i32x4*)(wp[i] + (in ? at : -kq * 16));
+        const i32x4 v = *(const i32x4*)(wp[i] + (in ? k : -kq * 16));
         a[u][i] = in ? v : i32x4{0, 0, 0, 0};
       }
-#pragma unroll
-      for (int j = 0; j < MT; ++j) b[u][j] = *(const i32x4*)(xp[j] + (in ? at : -kq * 16));
+      if constexpr (!FUSED) x_step(u, s);
     }
-    multiply();
+  };
+  auto multiply = [&](int s) {
+    if constexpr (FUSED) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) x_step(u, s);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][i], b[u], acc[i], 0, 0, 0);
+  };
+  fetch(wave);
+  if constexpr (FUSED) {
+    // M rows are shared out among the waves: all to one row, half to each of two, a quarter to each of three or four
+    static_assert(WAVES == 8 && I8_FUSED_ROWS == 4, "waves a row");
+    constexpr int VEC = gmk_elem<X>::VEC, KEEP = 2;
+    __shared__ float red[WAVES];
+    const int team = M == 1 ? 8 : M == 2 ? 4 : 2, m = wave / team, stride = team * 64 * VEC;
+    const int e0 = ((wave % team) * 64 + lane) * VEC;
+    const X* xr = x + (int64_t)min(m, M - 1) * Kx;
+    GmkMagnitude<X> mag;
+    gmk_u32x4 keep[KEEP];
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (e0 + i * stride < Kx) keep[i] = gmk_row_piece(xr, e0 + i * stride, Kx, 0.f);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (e0 + i * stride < Kx) mag.scan(keep[i]);
+    for (int e = e0 + KEEP * stride; e < Kx; e += stride) mag.scan(gmk_row_piece(xr, e, Kx, 0.f));
+    float mx = gmk_wave_max_all(mag.value());
+    if (lane == 0) red[wave] = mx;
+    __syncthreads();
+    for (int i = m * team; i < (m + 1) * team; ++i) mx = fmaxf(mx, red[i]);
+    const GmkQuant qu(mx);
+    if (m < M) {
+      auto put = [&](int e, const gmk_u32x4& v) {
+        unsigned w[2] = {0u, 0u};
+        if (e < Kx) qu.template piece<X>(v, w);
+        __builtin_memcpy(xlds + m * K + e, w, VEC);
+      };
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (e0 + i * stride < K) put(e0 + i * stride, keep[i]);
+      for (int e = e0 + KEEP * stride; e < K; e += stride) put(e, e < Kx ? gmk_row_piece(xr, e, Kx, 0.f) : gmk_u32x4{0u, 0u, 0u, 0u});
+      if (lane == 0) xs_row[m] = qu.scale();
+    }
+    __syncthreads();
+  }
+  for (int s = wave; s < steps; s += U * WAVES) {
+    multiply(s);
+    if (s + U * WAVES < steps) fetch(s + U * WAVES);
   }
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) part[(wave * NT * MT + i * MT + j) * 64 + lane] = acc[i][j];
+  for (int i = 0; i < NT; ++i) part[(wave * NT + i) * 64 + lane] = acc[i];
   __syncthreads();
-  for (int q = threadIdx.x; q < NT * MT * 64; q += 64 * WAVES) {
-    const int t = q >> 6, l = q & 63;
-    const int m = m0 + (t % MT) * 16 + (l & 15), n = n0 + (t / MT) * 16 + (l >> 4) * 4;
+  for (int q = threadIdx.x; q < NT * 64; q += 64 * WAVES) {
+    const int l = q & 63;
+    const int m = m0 + (l & 15), n = n0 + (q >> 6) * 16 + (l >> 4) * 4;
     if (m >= M || n >= N) continue;
-    const float xs = xscale[m];
+    const float xs = FUSED ? xs_row[FUSED ? m : 0] : xscale[m];
     float4 cs = make_float4(0.f, 0.f, 0.f, 0.f), cb = cs;
     float *sp = &cs.x, *bp = &cb.x;
 #pragma unroll
@@ -385,20 +423,21 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_i8_rows_kernel(const signed c
     }
     i32x4 v = part[q];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) v += part[w * NT * MT * 64 + q];
+    for (int w = 1; w < WAVES; ++w) v += part[w * NT * 64 + q];
     float4 z = i8_column(i8_scaled(v, xs), cs, cb), d;
     GMK_WITH_ACT(act, [&](auto f) { float4 a; f(z, a, d); z = a; });
     i8_put4<T>(z, y + (int64_t)m * N + n, N - n);
   }
 }
 
-template <class T, int MT, int NT, int WAVES, int U>
-static int gemm_i8_rows_launch(const signed char* xq, const float* xscale, const signed char* wq, const float* wscale, const float* bias,
-                               T* y, int M, int K, int N, int act, hipStream_t stream) {
-  const int64_t tm = (M + MT * 16 - 1) / (MT * 16), tn = (N + NT * 16 - 1) / (NT * 16);
-  GMK_REQUIRE(tm * tn < 0x7FFFFFFFll, GMK_E_TOO_LARGE);
-  hipLaunchKernelGGL((gemm_i8_rows_kernel<T, MT, NT, WAVES, U>), dim3((unsigned)(tm * tn)), dim3(64 * WAVES), 0, stream, xq, xscale, wq, wscale,
-                     bias, y, M, K, N, act, (int)tm);
+// Kx: columns of x where it is quantised here (K is then Kx rounded up to 16); else K
+template <class T, class X, int NT>
+static int gemm_i8_rows_launch(const X* x, const float* xscale, const signed char* wq, const float* wscale, const float* bias, T* y, int M,
+                               int K, int N, int act, int Kx, hipStream_t stream) {
+  const int64_t tm = (M + 15) / 16, tn = (N + NT * 16 - 1) / (NT * 16);
+  const int bytes = std::is_same<X, signed char>::value ? 0 : M * K;
+  hipLaunchKernelGGL((gemm_i8_rows_kernel<T, X, NT, 8, 4>), dim3((unsigned)(tm * tn)), dim3(512), bytes, stream, x, xscale, wq, wscale, bias, y, M,
+                     K, N, act, (int)tm, Kx);
   GMK_CHECK_LAUNCH();
   return GMK_OK;
 }
@@ -430,8 +469,9 @@ static int gemm_i8_launch(const signed char* xq, const float* xscale, const sign
   return gmk_with_dtype(ytype, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto f) { return f(xq, xscale, wq, wscale, bias, (T*)y, M, K, N, act, (hipStream_t)stream); };
-    if (tiles(16, 16) <= (M <= 16 ? 2 : 1) * cus) return go(gemm_i8_rows_launch<T, 1, 1, 8, 4>);
-    if (M <= 8) return go(gemm_i8_rows_launch<T, 1, 2, 8, 4>);
+    if (tiles(16, 16) <= (M <= 16 ? 2 : 1) * cus)
+      return gemm_i8_rows_launch<T, signed char, 1>(xq, xscale, wq, wscale, bias, (T*)y, M, K, N, act, K, (hipStream_t)stream);
+    if (M <= 8) return gemm_i8_rows_launch<T, signed char, 2>(xq, xscale, wq, wscale, bias, (T*)y, M, K, N, act, K, (hipStream_t)stream);
     if (tiles(32, 32) <= 2 * cus) return go(gemm_i8_tile_launch<T, 32, 32, 2, 2, 4>);
     if (M <= 32) return go(gemm_i8_tile_launch<T, 64, 32, 2, 2, 6>);
     const float e64 = estimate(64, 64, 2, 4.f, 0.38f), e128 = estimate(128, 128, 1, 6.5f, 0.47f);
@@ -444,11 +484,8 @@ static int gemm_i8_launch(const signed char* xq, const float* xscale, const sign
   });
 }
 
-extern "C" size_t gmk_gemm_i8_workspace_bytes(int M, int K, int N) { return 0; }
-
 extern "C" int gmk_gemm_i8(const signed char* xq, const float* xscale, const signed char* wq, const float* wscale,
-                           const float* bias, void* y, int ytype, int M, int K, int N, int act, void* ws, size_t ws_bytes,
-                           gmk_stream_t stream) {
+                           const float* bias, void* y, int ytype, int M, int K, int N, int act, gmk_stream_t stream) {
   const int rc = gemm_i8_check(M, K, N, ytype, act);
   if (rc != GMK_OK) return rc;
   GMK_REQUIRE(K % 16 == 0, GMK_E_SHAPE);
@@ -456,17 +493,19 @@ extern "C" int gmk_gemm_i8(const signed char* xq, const float* xscale, const sig
   GMK_REQUIRE(xq && xscale && wq && wscale && y, GMK_E_NULL);
   GMK_REQUIRE(gmk_aligned16(xq) && gmk_aligned16(wq) && gmk_aligned_to(xscale, 4) && gmk_aligned_to(wscale, 4) &&
               gmk_aligned_to(bias, 4) && gmk_aligned_to(y, gmk_dtype_size(ytype)), GMK_E_ALIGN);
-  GMK_REQUIRE(ws_bytes >= gmk_gemm_i8_workspace_bytes(M, K, N), GMK_E_WORKSPACE);
-  GMK_PLAN_HOOK(gmk_gemm_i8, xq, xscale, wq, wscale, bias, y, ytype, M, K, N, act, ws, ws_bytes, stream);
+  GMK_PLAN_HOOK(gmk_gemm_i8, xq, xscale, wq, wscale, bias, y, ytype, M, K, N, act, stream);
   return gemm_i8_launch(xq, xscale, wq, wscale, bias, y, ytype, M, K, N, act, stream);
 }
+
+// few rows are quantised by the product's own workgroups
+static bool linear_i8_fused(int M, int Kp) { return M <= I8_FUSED_ROWS && M * Kp <= I8_FUSED_BYTES; }
 
 // workspace of the linear layer: the quantised rows, then their scales
 static size_t linear_i8_q_bytes(int M, int K) { return (size_t)M * (size_t)((K + 15) / 16 * 16); }
 
 extern "C" size_t gmk_linear_i8_workspace_bytes(int M, int K, int N) {
-  if (M <= 0 || K <= 0 || N <= 0 || K > GMK_I8_MAX_K) return 0;
-  return linear_i8_q_bytes(M, K) + ((size_t)M * 4 + 15) / 16 * 16 + gmk_gemm_i8_workspace_bytes(M, (K + 15) / 16 * 16, N);
+  if (M <= 0 || K <= 0 || N <= 0 || K > GMK_I8_MAX_K || linear_i8_fused(M, (K + 15) / 16 * 16)) return 0;
+  return linear_i8_q_bytes(M, K) + (size_t)M * 4;
 }
 
 extern "C" int gmk_linear_i8_fwd(const void* x, int xtype, const signed char* wq, const float* wscale, const float* bias,
@@ -476,12 +515,22 @@ extern "C" int gmk_linear_i8_fwd(const void* x, int xtype, const signed char* wq
   if (rc != GMK_OK) return rc;
   GMK_REQUIRE(gmk_dtype_ok(xtype), GMK_E_UNSUPPORTED);
   if (M == 0) return GMK_OK;
-  GMK_REQUIRE(x && wq && wscale && y && ws, GMK_E_NULL);
+  GMK_REQUIRE(x && wq && wscale && y && (ws || linear_i8_fused(M, (K + 15) / 16 * 16)), GMK_E_NULL);
   GMK_REQUIRE(gmk_aligned_to(x, gmk_dtype_size(xtype)) && gmk_aligned16(wq) && gmk_aligned_to(wscale, 4) &&
               gmk_aligned_to(bias, 4) && gmk_aligned_to(y, gmk_dtype_size(ytype)) && gmk_aligned16(ws), GMK_E_ALIGN);
   GMK_REQUIRE(ws_bytes >= gmk_linear_i8_workspace_bytes(M, K, N), GMK_E_WORKSPACE);
   GMK_PLAN_HOOK(gmk_linear_i8_fwd, x, xtype, wq, wscale, bias, y, ytype, M, K, N, act, ws, ws_bytes, stream);
   const int Kp = (K + 15) / 16 * 16;
+  if (linear_i8_fused(M, Kp))
+    return gmk_with_dtype(ytype, [&](auto t) {
+      return gmk_with_dtype(xtype, [&](auto u) {
+        using T = decltype(t);
+        using X = decltype(u);
+        if ((N + 15) / 16 <= 2 * i8_cus())
+          return gemm_i8_rows_launch<T, X, 1>((const X*)x, nullptr, wq, wscale, bias, (T*)y, M, Kp, N, act, K, (hipStream_t)stream);
+        return gemm_i8_rows_launch<T, X, 2>((const X*)x, nullptr, wq, wscale, bias, (T*)y, M, Kp, N, act, K, (hipStream_t)stream);
+      });
+    });
   signed char* q = (signed char*)ws;
   float* s = (float*)(q + linear_i8_q_bytes(M, K));
   const int e = gmk_quantize_rows_launch(x, xtype, q, s, M, K, Kp, stream);

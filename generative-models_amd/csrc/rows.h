@@ -64,14 +64,21 @@ __device__ __forceinline__ gmk_u32x4 gmk_pack(const float* f) {
 }
 
 // The piece of a row that starts at element e: whole pieces in one load, the last, partial one element by element, its
-// missing elements -inf (what leaves a maximum and a sum of exponentials as they are).
+// missing elements `fill` (-inf leaves a maximum and a sum of exponentials as they are, 0 a largest magnitude).
 template <class T>
-__device__ __forceinline__ gmk_u32x4 gmk_row_piece(const T* row, int64_t e, int64_t C) {
+__device__ __forceinline__ gmk_u32x4 gmk_row_piece(const T* row, int64_t e, int64_t C, float fill = -__builtin_inff()) {
   constexpr int VEC = gmk_elem<T>::VEC;
   if (e + VEC <= C) return gmk_load16(row + e);
   T t[VEC];
+  if (e >= C) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) t[i] = e + i < C ? row[e + i] : (T)(-__builtin_inff());
+    for (int i = 0; i < VEC; ++i) t[i] = (T)fill;
+    gmk_u32x4 v;
+    __builtin_memcpy(&v, t, 16);
+    return v;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) t[i] = e + i < C ? row[e + i] : (T)fill;
   gmk_u32x4 v;
   __builtin_memcpy(&v, t, 16);
   return v;

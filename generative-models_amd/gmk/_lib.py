@@ -66,8 +66,7 @@ SIGNATURES = {
     "gmk_vae_loss_fwd_bwd_fused": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _L, _L, _F, _I, _P, _Z, _P, _P]),
     "gmk_vae_loss_eval": (_I, [_P, _P, _P, _P, _P, _L, _L, _L, _F, _I, _P, _Z, _P]),
     "gmk_quantize_rows": (_I, [_P, _I, _P, _P, _L, _I, _I, _P]),
-    "gmk_gemm_i8_workspace_bytes": (_Z, [_I, _I, _I]),
-    "gmk_gemm_i8": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _Z, _P]),
+    "gmk_gemm_i8": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "gmk_linear_i8_workspace_bytes": (_Z, [_I, _I, _I]),
     "gmk_linear_i8_fwd": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "gmk_topk_rows_workspace_bytes": (_Z, [_L, _L, _I]),

@@ -626,9 +626,8 @@ def matmul_i8(xq, xscale, wq, wscale, bias=None, act=None, out_dtype=torch.float
     _chk_rows("xscale", xscale, _FP32, (M,), dev)
     N = _i8_args(dev, K, wq, wscale, bias, out_dtype)
     y = _new((M, N), xq.device, out_dtype)
-    ws, nbytes = _scratch(xq.device, "gmk_gemm_i8_workspace_bytes", M, K, N)
     check(lib().gmk_gemm_i8(_p(xq), _p(xscale), _p(wq), _p(wscale), _p(bias), _p(y), _FLOAT_IDS[out_dtype], M, K, N, act_id(act),
-                            _p(ws), nbytes, _stream_of(dev)))
+                            _stream_of(dev)))
     return y
 
 

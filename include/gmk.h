@@ -337,14 +337,14 @@ int gmk_quantize_rows(const void* x, int xtype, signed char* q, float* scale, in
 
 /* gmk_gemm_i8: y (M,N) = act((sum_k xq[m][k] wq[n][k]) * xscale[m] * wscale[n] + bias[n]), the sum exact in 32-bit
  *   integers.  xq (M,K), wq (N,K) int8 in [-128, 127], K % 16 == 0 (rows that gmk_quantize_rows padded are whole), K <= GMK_I8_MAX_K;
- *   bias (N) fp32 or NULL; act: enum gmk_act.  ws >= gmk_gemm_i8_workspace_bytes(M, K, N) bytes. */
+ *   bias (N) fp32 or NULL; act: enum gmk_act. */
 #define GMK_I8_MAX_K 131056
-size_t gmk_gemm_i8_workspace_bytes(int M, int K, int N);
 int gmk_gemm_i8(const signed char* xq, const float* xscale, const signed char* wq, const float* wscale, const float* bias,
-                void* y, int ytype, int M, int K, int N, int act, void* ws, size_t ws_bytes, gmk_stream_t stream);
+                void* y, int ytype, int M, int K, int N, int act, gmk_stream_t stream);
 /* gmk_linear_i8_fwd: the same from floating activations: x (M,K) is quantised row by row as gmk_quantize_rows does, and
  *   wq (N, ldw) holds the weight's rows as gmk_quantize_rows wrote them once, ldw = K rounded up to 16.  K <= GMK_I8_MAX_K.
- *   The 8-bit counterpart of gmk_linear_fwd, for inference (no derivative).  ws >= gmk_linear_i8_workspace_bytes(M, K, N). */
+ *   The 8-bit counterpart of gmk_linear_fwd, for inference (no derivative).  ws >= gmk_linear_i8_workspace_bytes(M, K, N) bytes
+ *   (0 for a few rows: NULL is fine). */
 size_t gmk_linear_i8_workspace_bytes(int M, int K, int N);
 int gmk_linear_i8_fwd(const void* x, int xtype, const signed char* wq, const float* wscale, const float* bias, void* y,
                       int ytype, int M, int K, int N, int act, void* ws, size_t ws_bytes, gmk_stream_t stream);

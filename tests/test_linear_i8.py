@@ -80,7 +80,7 @@ def test_quantize_rows_halves_extremes_and_rows_without_a_scale():
 
 
 # M, K, N: single rows, few rows, tiles that end inside, K chunks that end inside, odd everything, several tiles each way
-SHAPES = [(1, 16, 1), (1, 256, 10), (1, 4096, 1000), (2, 100, 37), (4, 8200, 33), (5, 1, 5), (8, 4097, 129), (16, 640, 64), (17, 64, 17), (24, 8192, 200),
+SHAPES = [(1, 30000, 40), (4, 8192, 9000), (3, 10, 9001), (1, 16, 1), (1, 256, 10), (1, 4096, 1000), (2, 100, 37), (4, 8200, 33), (5, 1, 5), (8, 4097, 129), (16, 640, 64), (17, 64, 17), (24, 8192, 200),
           (33, 2050, 1030), (64, 16384, 48), (65, 128, 257), (100, 333, 300), (128, 256, 128), (129, 1357, 131), (256, 4096, 256), (257, 144, 513), (300, 80, 1100),
           (512, 512, 512), (777, 1357, 503), (1030, 272, 770)]
 
@@ -162,7 +162,7 @@ def test_gemm_i8_larger_kernels(shape):
 
 
 @gpu
-@pytest.mark.parametrize("M", [1, 20, 150])
+@pytest.mark.parametrize("M", [1, 4, 20, 150])
 def test_linear_i8_rows_are_independent_and_nan_stays_in_its_row(M):
     from gmk import ops
     K, N = 513, 77
@@ -205,7 +205,7 @@ def test_linear_i8_writes_its_rows_only_and_reads_only_its_own():
         xb[32: 32 + M * K] = _randn(4, M * K).cuda()
         yb = torch.full((M * N + 64,), 7.0, device="cuda")
         x, y = xb[32: 32 + M * K].view(M, K), yb[32: 32 + M * N].view(M, N)
-        scratch = torch.empty(int(lib().gmk_linear_i8_workspace_bytes(M, K, N)), dtype=torch.uint8, device="cuda")
+        scratch = torch.empty(int(lib().gmk_linear_i8_workspace_bytes(M, K, N)) + 16, dtype=torch.uint8, device="cuda")
         check(lib().gmk_linear_i8_fwd(x.data_ptr(), 0, wq.data_ptr(), ws.data_ptr(), None, y.data_ptr(), 0, M, K, N, 0, scratch.data_ptr(),
                                       scratch.numel(), torch.cuda.current_stream().cuda_stream))
         assert torch.equal(y, ops.linear_i8(x.clone(), wq, ws))
@@ -275,21 +275,21 @@ def test_c_entries_refuse_bad_arguments():
     assert q(x=None) == q(q=None) == q(s=None) == E["null"]
     assert q(x=odd) == q(q=ctypes.c_void_p(4100)) == q(s=odd) == E["align"]
     assert q(M=0, x=None) == 0
-    g = lambda **k: h.gmk_gemm_i8(*{**dict(xq=p, xs=p, wq=p, ws=p, b=None, y=p, yt=0, M=2, K=32, N=3, act=0, w=p, wb=1 << 40, st=None), **k}.values())  # noqa: E731
+    g = lambda **k: h.gmk_gemm_i8(*{**dict(xq=p, xs=p, wq=p, ws=p, b=None, y=p, yt=0, M=2, K=32, N=3, act=0, st=None), **k}.values())  # noqa: E731
     assert g(yt=9) == g(act=9) == g(act=-1) == E["unsupported"]
     assert g(M=-1) == g(K=0) == g(K=20) == g(N=0) == E["shape"]
     assert g(K=131072) == E["large"]
     assert g(xq=None) == g(xs=None) == g(wq=None) == g(ws=None) == g(y=None) == E["null"]
     assert g(xq=ctypes.c_void_p(4104)) == g(wq=ctypes.c_void_p(4104)) == g(b=odd) == g(y=odd) == E["align"]
     assert g(M=0) == 0
-    f = lambda **k: h.gmk_linear_i8_fwd(*{**dict(x=p, xt=0, wq=p, ws=p, b=None, y=p, yt=0, M=2, K=20, N=3, act=0, w=p, wb=1 << 40, st=None), **k}.values())  # noqa: E731
+    f = lambda **k: h.gmk_linear_i8_fwd(*{**dict(x=p, xt=0, wq=p, ws=p, b=None, y=p, yt=0, M=20, K=20, N=3, act=0, w=p, wb=1 << 40, st=None), **k}.values())  # noqa: E731
     assert f(xt=5) == f(yt=5) == f(act=12) == E["unsupported"]
     assert f(M=-2) == f(K=-1) == f(N=0) == E["shape"]
     assert f(K=131057) == E["large"]
     assert f(x=None) == f(w=None) == f(y=None) == E["null"]
     assert f(x=odd) == f(w=ctypes.c_void_p(4104)) == E["align"]
-    assert f(wb=int(h.gmk_linear_i8_workspace_bytes(2, 20, 3)) - 1) == E["workspace"]
-    assert h.gmk_linear_i8_workspace_bytes(2, 20, 3) >= 2 * 32 + 8
+    assert f(wb=int(h.gmk_linear_i8_workspace_bytes(20, 20, 3)) - 1) == E["workspace"]
+    assert h.gmk_linear_i8_workspace_bytes(20, 20, 3) >= 20 * 32 + 80
 
 
 @gpu
