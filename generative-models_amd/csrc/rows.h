@@ -96,6 +96,12 @@ __device__ __forceinline__ float gmk_wave_max_all(float v) {   // NaN-free maxim
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
   return v;
 }
+// Maximum that is NaN where any value is.
+__device__ __forceinline__ float gmk_wave_maximum_all(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = __builtin_elementwise_maximum(v, __shfl_xor(v, o, 64));
+  return v;
+}
 __device__ __forceinline__ float gmk_wave_sum_all(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -114,6 +120,18 @@ __device__ __forceinline__ float gmk_block_max_all(float v, float* red) {
   float r = red[0];
 #pragma unroll
   for (int i = 1; i < NT / 64; ++i) r = fmaxf(r, red[i]);
+  return r;
+}
+template <int NT>
+__device__ __forceinline__ float gmk_block_maximum_all(float v, float* red) {
+  v = gmk_wave_maximum_all(v);
+  if constexpr (NT == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float r = red[0];
+#pragma unroll
+  for (int i = 1; i < NT / 64; ++i) r = __builtin_elementwise_maximum(r, red[i]);
   return r;
 }
 template <int NT>
