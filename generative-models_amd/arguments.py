@@ -40,4 +40,12 @@ def get_args_parser(add_help=True):
     # not in the reference: time the train step with both kernel paths of the 3-channel-side layers on this device
     # and keep the faster one (gmk/tune.py); off by default so that runs stay bitwise comparable across devices
     a("--tune_kernels", dest="tune_kernels", help="per-device kernel-path tuning before training", action="store_true")
+    # not in the reference: train the classifier of the metrics from another one (models/classifiers.py), whose two fully
+    # connected layers may answer in 8-bit integers
+    a("--teacher_checkpoint", default=None, type=str, help="path to a full-model classifier to distil from")
+    a("--teacher_int8", dest="teacher_int8", help="teacher's fully connected layers in 8-bit integers", action="store_true")
+    a("--distill_topk", default=3, type=int, help="logits of the teacher that are kept for each sample")
+    a("--distill_t", default=4.0, type=float, help="distillation temperature")
+    a("--distill_soft", default=0.9, type=float, help="weight of the teacher's part of the loss")
+    a("--distill_hard", default=0.1, type=float, help="weight of the labels' part of the loss")
     return parser

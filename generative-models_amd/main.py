@@ -153,8 +153,12 @@ def main(args):
             print(f'\n\nCIFAR-10 Test Accuracy {test_acc:.2f}')
         else:
             print(f'\n\nClassifier checkpoint is not found at {classifier_checkpoint}')
+            teacher = None
+            if args.teacher_checkpoint is not None:
+                teacher = torch.load(args.teacher_checkpoint, map_location=device, weights_only=False)
+                teacher.int8_fc = args.teacher_int8
             classifier = train_classifier(args, classifier=None, train_dataloader=train_dataloader,
-                                          test_dataloader=test_dataloader, device=device)
+                                          test_dataloader=test_dataloader, device=device, teacher=teacher)
         if isinstance(plain_ae, dict) or isinstance(classifier, dict):
             raise NotImplementedError('\n\nmodel checkpoint must be a full saved model, not a state_dict\n\n')
     else:

@@ -12,6 +12,9 @@ Two forward paths, chosen by the module's mode:
   3 implicit-GEMM convs, 3 max-pools and 2 GEMMs.  CUDA tensors only (no CPU path).
 * train mode (train_classifier, an auxiliary model's training loop: out of the hot-path scope):
   ordinary PyTorch modules under autograd.
+
+Beyond the reference, a classifier can learn from another one (train_classifier(teacher=...), distillation_loss) and answer with its two
+fully connected layers in 8-bit integers (int8_fc): both run on libgmk.
 """
 import numpy as np
 import torch
@@ -22,6 +25,9 @@ from utils import print_debug
 
 
 class Classifier(nn.Module):
+    # eval mode: fc and fc_out in 8-bit integers, one scale for each sample and each output (gmk.ops.linear_i8); set it on an instance
+    int8_fc = False
+
     def __init__(self, args=None) -> None:
         super().__init__()
         self.debug = args.debug
@@ -45,7 +51,7 @@ class Classifier(nn.Module):
         bn(conv(x)) = conv(x; w * s) + (b - mean) * s + beta,  s = gamma / sqrt(var + eps).
         Cached until a parameter or buffer is modified in place (tensor version counters) or replaced."""
         tensors = list(self.parameters()) + list(self.buffers())
-        key = tuple((t.data_ptr(), t._version) for t in tensors)
+        key = (self.int8_fc,) + tuple((t.data_ptr(), t._version) for t in tensors)
         cache = self.__dict__.get("_gmk_fold")
         if cache is not None and cache[0] == key:
             return cache[1]
@@ -56,6 +62,11 @@ class Classifier(nn.Module):
                 w = layer.weight * s.view(-1, *([1] * (layer.weight.dim() - 1)))
                 b = (layer.bias - bn.running_mean) * s + bn.bias
                 out[layer] = (w.float().contiguous(), b.float().contiguous())
+            out[self.fc_out] = (self.fc_out.weight.detach().float().contiguous(), self.fc_out.bias.detach().float().contiguous())
+            if self.int8_fc:
+                for layer in (self.fc, self.fc_out):
+                    w, b = out[layer]
+                    out[layer] = (*ops.quantize_rows(w), b)
         self.__dict__["_gmk_fold"] = (key, out)
         return out
 
@@ -71,10 +82,10 @@ class Classifier(nn.Module):
             x = ops.conv2d_fwd(x, w, b, stride=1, act=a)       # conv + folded BN + activation, classifiers.py:33,37,42
             x = ops.maxpool2_fwd(x, want_idx=False)            # :35,39,44
         x = x.view(-1, 4 * 4 * 256)                            # :46
-        w, b = f[self.fc]
-        x = ops.linear_fwd(x, w, b, act=a)                     # fc + folded BN1d + activation, :48 (dropout: identity in eval)
+        linear = ops.linear_i8 if self.int8_fc else ops.linear_fwd
+        x = linear(x, *f[self.fc], act=a)                      # fc + folded BN1d + activation, :48 (dropout: identity in eval)
         self.latent_vector = x                                 # :51
-        return ops.linear_fwd(x, self.fc_out.weight.detach(), self.fc_out.bias.detach())  # :52
+        return linear(x, *f[self.fc_out])                      # :52
 
     # ------------------------------------------------------------------ train: PyTorch autograd (out of scope for libgmk)
     def _forward_torch(self, x):
@@ -99,6 +110,33 @@ class Classifier(nn.Module):
         return state
 
 
+class _DistillFn(torch.autograd.Function):
+    """Row losses of gmk.ops.distill_fwd with distill_bwd as their gradient; the teacher's side and the labels have none."""
+
+    @staticmethod
+    def forward(ctx, logits, value, index, labels, T, soft, hard):
+        loss, stats = ops.distill_fwd(logits, value, index, labels, T, soft, hard)
+        ctx.save_for_backward(logits, value, index, labels, stats)
+        ctx.weights = (T, soft, hard)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        logits, value, index, labels, stats = ctx.saved_tensors
+        dz = ops.distill_bwd(grad.float().contiguous(), logits, value, index, labels, stats, *ctx.weights)
+        return dz, None, None, None, None, None, None
+
+
+def distillation_loss(outputs, value, index, labels=None, T=4.0, soft=0.9, hard=0.1):
+    """Loss of each sample (n,) of a student's logits (n, C): soft T^2 KL(teacher || student) at temperature T over the teacher's kept logits
+    `value` (n, k) of the classes `index` (n, k) int32 (gmk.ops.topk_rows; -1: no entry), plus hard * cross entropy where labels (n,) are
+    given (outside [0, C): none).  CUDA tensors; outputs fp32, bf16 or fp16, under autograd."""
+    if labels is None:
+        hard = 0.0
+    return _DistillFn.apply(outputs.contiguous(), value.detach(), index, labels, float(T), float(soft), float(hard))
+
+
 def compute_accuracy(outputs, labels):
     """Top-1 accuracy of a batch in percent (same value as reference classifiers.py:69-74)."""
     with torch.no_grad():
@@ -107,29 +145,42 @@ def compute_accuracy(outputs, labels):
 
 
 def _epoch_accuracy(classifier, dataloader, device, step=None):
-    """Mean of the per-batch accuracies over one pass; `step(outputs, labels)` runs the optimisation when given."""
+    """Mean of the per-batch accuracies over one pass; `step(outputs, labels, images)` runs the optimisation when given."""
     accs = []
     for images, labels in dataloader:
         images, labels = images.to(device), labels.to(device)
         outputs = classifier(images)
         if step is not None:
-            step(outputs, labels)
+            step(outputs, labels, images)
         accs.append(compute_accuracy(outputs, labels))
     return np.mean(accs)
 
 
-def train_classifier(args, classifier=None, train_dataloader=None, test_dataloader=None, device=None):
+def train_classifier(args, classifier=None, train_dataloader=None, test_dataloader=None, device=None, teacher=None):
     """Auxiliary model training (reference classifiers.py:77-113): cross entropy, AdamW, cosine LR stepped every
-    iteration over epochs * len(loader) steps; the full model object is saved, as the metrics' loader expects."""
+    iteration over epochs * len(loader) steps; the full model object is saved, as the metrics' loader expects.
+    With a `teacher` (any module of logits; not in the reference) the student learns from its args.distill_topk largest logits of each
+    sample and the labels (distillation_loss, temperature args.distill_t, weights args.distill_soft and args.distill_hard)."""
     print('\n\nTraining CIFAR-10 Classifier\n\n')
     classifier = Classifier(args=args).to(device) if classifier is None else classifier
     optim = torch.optim.AdamW(classifier.parameters(), lr=args.lr, weight_decay=args.wd)
     sched = torch.optim.lr_scheduler.CosineAnnealingLR(optimizer=optim, T_max=args.epochs * len(train_dataloader))
     criterion = nn.CrossEntropyLoss()
+    if teacher is not None:
+        teacher = teacher.to(device).eval()
 
-    def step(outputs, labels):
+    def loss_of(outputs, labels, images):
+        if teacher is None:
+            return criterion(outputs, labels)
+        with torch.no_grad():
+            logits = teacher(images).contiguous()
+            value, index = ops.topk_rows(logits, min(getattr(args, "distill_topk", 3), logits.shape[1]))
+        return distillation_loss(outputs, value, index, labels, T=getattr(args, "distill_t", 4.0), soft=getattr(args, "distill_soft", 0.9),
+                                 hard=getattr(args, "distill_hard", 0.1)).mean()
+
+    def step(outputs, labels, images):
         optim.zero_grad()
-        criterion(outputs, labels).backward()
+        loss_of(outputs, labels, images).backward()
         optim.step()
         sched.step()
 

@@ -1,0 +1,182 @@
+"""A classifier from another one: the 8-bit fully connected layers of Classifier, distillation_loss under autograd, train_classifier with
+a teacher, and its command-line flags."""
+import math
+import os
+import types
+
+import pytest
+import torch
+
+from test_linear_i8 import _linear_oracle
+
+gpu = pytest.mark.gpu
+
+
+def _randn(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+def _classifier(seed=0, latent=64, act="gelu", **more):
+    from models.classifiers import Classifier
+    from utils import get_activation_function
+    torch.manual_seed(seed)
+    args = types.SimpleNamespace(debug=False, latent_size=latent, dropout=0.0, act_fn=get_activation_function(act), lr=1e-3, wd=0.0, epochs=1, **more)
+    return Classifier(args=args), args
+
+
+@gpu
+@pytest.mark.parametrize("batch", [1, 50, 256])
+def test_int8_classifier_layers(monkeypatch, batch):
+    """Both layers of the 8-bit forward against 64 bits, from their own inputs; the folded weights are quantised once and again after an
+    update; switching back gives the fp32 answers bit for bit."""
+    from gmk import ops
+    m, _ = _classifier()
+    m = m.cuda().eval()
+    x = torch.rand(batch, 3, 32, 32, generator=torch.Generator().manual_seed(batch)).cuda()
+    plain = m(x)
+    seen, quantised = [], []
+    real, realq = ops.linear_i8, ops.quantize_rows
+    monkeypatch.setattr(ops, "linear_i8", lambda x, wq, ws, b, act=None: seen.append((x, wq, ws, b, act, real(x, wq, ws, b, act=act))) or seen[-1][-1])
+    monkeypatch.setattr(ops, "quantize_rows", lambda w: quantised.append(w) or realq(w))
+    m.int8_fc = True
+    y = m(x)
+    assert len(seen) == 2 and len(quantised) == 2 and y is seen[1][-1] and m.latent_vector is seen[0][-1]
+    for xi, wq, ws, b, act, out in seen:
+        ref, z = _linear_oracle(xi.cpu(), wq.cpu(), ws.cpu(), b.cpu(), "gelu" if act else None)
+        tol = (4 * 1.13 + 8) * 2.0 ** -24 * (z.abs() + b.abs().cpu()) + 1.5e-7 * z.abs() + 1e-37   # as in test_linear_i8
+        assert ((out.cpu().double() - ref).abs() <= tol).all()
+    # rows of x and of w lose at most half a step each: |error of the sum| <= sum |x| sw / 2 + |w| sx / 2 + sx sw / 4
+    xi, wq, ws, b, _, out = seen[1]
+    w = m.fc_out.weight.detach().double().cpu()
+    sx = xi.cpu().double().abs().amax(1, keepdim=True) / 127
+    sw = ws.cpu().double()
+    full = xi.cpu().double() @ w.T + b.cpu().double()
+    bound = xi.cpu().double().abs().sum(1, keepdim=True) * sw / 2 + sx / 2 * w.abs().sum(1) + sx * sw / 4 * w.shape[1]
+    assert ((out.cpu().double() - full).abs() <= bound * 1.001 + 1e-5).all()
+    m(x)
+    assert len(quantised) == 2
+    with torch.no_grad():
+        m.fc_out.weight.mul_(2.0)
+    m(x)
+    assert len(quantised) == 4
+    with torch.no_grad():
+        m.fc_out.weight.mul_(0.5)
+    m.int8_fc = False
+    assert torch.equal(m(x), plain)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distillation_loss_gradient(dtype):
+    """The gradient through autograd, with different weights of the samples, against automatic differentiation in 64 bits."""
+    from models.classifiers import distillation_loss
+    n, C, k, T, soft, hard = 40, 30, 5, 3.0, 0.7, 0.3
+    z, w = _randn(1, n, C).to(dtype), _randn(2, n)
+    t, idx = (3 * _randn(3, n, C)).topk(k, dim=1)
+    idx = idx.int()
+    idx[::4, 2:] = -1
+    labels = torch.randint(0, C, (n,), generator=torch.Generator().manual_seed(4))
+    labels[::5] = -100
+    a = z.cuda().requires_grad_(True)
+    loss = distillation_loss(a, t.cuda(), idx.cuda(), labels.cuda(), T, soft, hard)
+    (loss * w.cuda()).sum().backward()
+    x = z.double().requires_grad_(True)
+    keep = idx >= 0
+    at = idx.long().clamp(min=0)
+    p = torch.log_softmax((t.double() / T).masked_fill(~keep, -math.inf), 1)
+    q = torch.log_softmax(x / T, 1).gather(1, at)
+    ref = soft * T * T * (p.exp() * (p - q).masked_fill(~keep, 0)).nan_to_num(0).sum(1)
+    ref = ref + hard * torch.nn.functional.cross_entropy(x, labels, reduction="none", ignore_index=-100)
+    (ref * w.double()).sum().backward()
+    eps = torch.finfo(dtype).eps / 2
+    assert loss.dtype == torch.float32 and a.grad.dtype == dtype
+    # loss: sums of C terms of |d / T| up to 4: about 60 roundings of 2^-24 of values up to 10; gradient the same, and its output rounding
+    assert (loss.detach().cpu().double() - ref.detach()).abs().max() < 600 * 2.0 ** -24
+    assert ((a.grad.cpu().double() - x.grad).abs() <= eps * x.grad.abs() + 100 * 2.0 ** -24 * w.double().abs()[:, None] * (1 + eps)).all()
+    # without labels; a strided view of the logits; no gradient asked
+    b = z.cuda()
+    plain = distillation_loss(b, t.cuda(), idx.cuda(), None, T, soft, hard)
+    wide = torch.empty(n, 2 * C, dtype=dtype, device="cuda")
+    wide[:, ::2] = b
+    assert torch.equal(distillation_loss(wide[:, ::2], t.cuda(), idx.cuda(), None, T, soft), plain) and not plain.requires_grad
+
+
+@gpu
+def test_distillation_step_in_a_graph():
+    """Loss and gradient captured and replayed on new logits, with eager work of other leaves between the replays."""
+    from models.classifiers import distillation_loss
+    n, C, k = 64, 10, 3
+    t, idx = (v.cuda() for v in _randn(1, n, C).topk(k, dim=1))
+    idx = idx.int()
+    labels = torch.randint(0, C, (n,), generator=torch.Generator().manual_seed(2)).cuda()
+    ones = torch.full((n,), 1.0 / n, device="cuda")
+
+    def eager(z):
+        z = z.clone().requires_grad_(True)
+        loss = distillation_loss(z, t, idx, labels)
+        return loss.detach(), torch.autograd.grad(loss, z, ones)[0]
+
+    static = torch.zeros(n, C, device="cuda", requires_grad=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(distillation_loss(static, t, idx, labels), static, ones)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loss = distillation_loss(static, t, idx, labels)
+        grad = torch.autograd.grad(loss, static, ones)[0]
+    for i in range(3):
+        z = _randn(10 + i, n, C).cuda()
+        with torch.no_grad():
+            static.copy_(z)
+        g.replay()
+        torch.cuda.synchronize()
+        want = eager(z)
+        assert torch.equal(loss.detach(), want[0]) and torch.equal(grad, want[1])
+
+
+@gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_train_classifier_with_a_teacher(tmp_path, monkeypatch, int8):
+    """One epoch of two batches from a teacher: it runs, the student moves, the teacher does not, and the first step's loss is the
+    definition's."""
+    from models import classifiers
+    monkeypatch.chdir(tmp_path)
+    os.makedirs("checkpoints")
+    teacher, _ = _classifier(1)
+    teacher.int8_fc = int8
+    student, args = _classifier(2, distill_topk=4, distill_t=2.0, distill_soft=0.8, distill_hard=0.2)
+    student, teacher = student.cuda(), teacher.cuda()
+    before = {k: v.clone() for k, v in teacher.state_dict().items()}
+    first = {k: v.clone() for k, v in student.state_dict().items()}
+    g = torch.Generator().manual_seed(3)
+    data = [(torch.rand(16, 3, 32, 32, generator=g), torch.randint(0, 10, (16,), generator=g)) for _ in range(2)]
+    losses = []
+    real = classifiers.distillation_loss
+    monkeypatch.setattr(classifiers, "distillation_loss", lambda z, v, i, l, **k: losses.append((z.detach().clone(), v, i, l, k, real(z, v, i, l, **k))) or losses[-1][-1])
+    out = classifiers.train_classifier(args, student, data, data, torch.device("cuda"), teacher=teacher)
+    assert out is student and len(losses) == 2
+    z, v, i, l, kw, loss = losses[0]
+    assert v.shape == (16, 4) and i.dtype == torch.int32 and kw == dict(T=2.0, soft=0.8, hard=0.2)
+    with torch.no_grad():
+        logits = teacher.eval()(data[0][0].cuda())
+    assert torch.equal(i.long(), torch.sort(logits.double(), dim=1, descending=True, stable=True)[1][:, :4])
+    z, v = z.double().cpu(), v.double().cpu()
+    p = torch.log_softmax(v / 2, 1)
+    kl = (p.exp() * (p - torch.log_softmax(z / 2, 1).gather(1, i.long().cpu()))).sum(1)
+    ref = 0.8 * 4 * kl + 0.2 * torch.nn.functional.cross_entropy(z, l.cpu(), reduction="none")
+    assert (loss.detach().cpu().double() - ref).abs().max() < 200 * 2.0 ** -24 * (1 + z.abs().max())
+    assert all(torch.equal(v, before[k]) for k, v in teacher.state_dict().items())
+    assert any(not torch.equal(v, first[k]) for k, v in student.state_dict().items())
+    assert os.path.isfile("checkpoints/cifar_classifier_64.pth")
+    again = torch.load("checkpoints/cifar_classifier_64.pth", weights_only=False)
+    assert not again.int8_fc and "_gmk_fold" not in again.__dict__
+
+
+def test_flags():
+    from arguments import get_args_parser
+    a = get_args_parser().parse_args([])
+    assert a.teacher_checkpoint is None and not a.teacher_int8 and (a.distill_topk, a.distill_t, a.distill_soft, a.distill_hard) == (3, 4.0, 0.9, 0.1)
+    a = get_args_parser().parse_args("--teacher_checkpoint t.pth --teacher_int8 --distill_topk 5 --distill_t 2".split())
+    assert a.teacher_checkpoint == "t.pth" and a.teacher_int8 and a.distill_topk == 5 and a.distill_t == 2.0
