@@ -388,8 +388,8 @@ extern "C" size_t gmk_distill_workspace_bytes(int64_t n, int64_t C) {
 
 static int distill_check(int ztype, int ttype, int64_t n, int64_t C, int k, float T, float soft, float hard) {
   GMK_REQUIRE(gmk_dtype_ok(ztype) && gmk_dtype_ok(ttype), GMK_E_UNSUPPORTED);
-  GMK_REQUIRE(T > 0.f && T < __builtin_inff() && soft - soft == 0.f && hard - hard == 0.f, GMK_E_UNSUPPORTED);
-  GMK_REQUIRE(n >= 0 && n <= GMK_MAX_ROWS && C > 0 && k > 0, GMK_E_SHAPE);
+  GMK_REQUIRE(T >= GMK_DISTILL_MIN_T && T <= GMK_DISTILL_MAX_T && soft - soft == 0.f && hard - hard == 0.f, GMK_E_UNSUPPORTED);
+  GMK_REQUIRE(n >= 0 && C > 0 && k > 0, GMK_E_SHAPE);
   GMK_REQUIRE(k <= GMK_DISTILL_MAX_K && C < 0x7FFFFFFFll, GMK_E_TOO_LARGE);
   return GMK_OK;
 }
@@ -411,7 +411,7 @@ static int distill_launch(const void* z, int ztype, const DistillArgs& a, const 
     constexpr int VEC = gmk_elem<T>::VEC;
     if (distill_in_parts(MODE, n, a.C, VEC)) {
       const int64_t parts = distill_parts(a.C, VEC);
-      GMK_REQUIRE(n * parts <= GMK_MAX_ROWS, GMK_E_TOO_LARGE);
+      GMK_REQUIRE(gmk_grid_ok(n * parts, DISTILL_NT), GMK_E_TOO_LARGE);
       hipLaunchKernelGGL((distill_part_kernel<T>), dim3((unsigned)(n * parts)), dim3(DISTILL_NT), 0, stream, (const T*)z, a, weight, (float*)ws, (unsigned)parts);
       GMK_CHECK_LAUNCH();
       constexpr int NT = MODE == 0 ? 64 : DISTILL_NT;   // the loss alone is a wave's work
@@ -420,16 +420,19 @@ static int distill_launch(const void* z, int ztype, const DistillArgs& a, const 
       GMK_CHECK_LAUNCH();
       return GMK_OK;
     }
-    auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads), 0, stream, (const T*)z, a, weight, scale, loss, stats, (T*)dz); };
+    auto go = [&](auto kernel, int threads) -> int {
+      GMK_REQUIRE(gmk_grid_ok(n, threads), GMK_E_TOO_LARGE);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads), 0, stream, (const T*)z, a, weight, scale, loss, stats, (T*)dz);
+      GMK_CHECK_LAUNCH();
+      return GMK_OK;
+    };
     const int64_t pieces = (a.C + VEC - 1) / VEC;
-    if (pieces <= 64) go(distill_row_kernel<T, 64, 1, MODE>, 64);
-    else if (pieces <= 256) go(distill_row_kernel<T, 64, 4, MODE>, 64);
-    else if (pieces <= 1024) go(distill_row_kernel<T, 256, 4, MODE>, 256);
-    else if (pieces <= 2048) go(distill_row_kernel<T, 256, 8, MODE>, 256);
-    else if (pieces <= 4096) go(distill_row_kernel<T, 512, 8, MODE>, 512);
-    else go(distill_row_kernel<T, 1024, 8, MODE>, 1024);
-    GMK_CHECK_LAUNCH();
-    return GMK_OK;
+    if (pieces <= 64) return go(distill_row_kernel<T, 64, 1, MODE>, 64);
+    if (pieces <= 256) return go(distill_row_kernel<T, 64, 4, MODE>, 64);
+    if (pieces <= 1024) return go(distill_row_kernel<T, 256, 4, MODE>, 256);
+    if (pieces <= 2048) return go(distill_row_kernel<T, 256, 8, MODE>, 256);
+    if (pieces <= 4096) return go(distill_row_kernel<T, 512, 8, MODE>, 512);
+    return go(distill_row_kernel<T, 1024, 8, MODE>, 1024);
   });
 }
 
@@ -440,7 +443,7 @@ static int distill_bwd_launch(const void* z, int ztype, const DistillArgs& a, co
     constexpr int VEC = gmk_elem<T>::VEC;
     const bool small = a.C <= 64 * DISTILL_KEEP * VEC;
     const int64_t parts = small ? 1 : distill_parts(a.C, VEC);
-    GMK_REQUIRE(n * parts <= GMK_MAX_ROWS, GMK_E_TOO_LARGE);
+    GMK_REQUIRE(gmk_grid_ok(n * parts, DISTILL_NT), GMK_E_TOO_LARGE);
     if (small) hipLaunchKernelGGL((distill_grad_kernel<T, 64, 1>), dim3((unsigned)n), dim3(64), 0, stream, (const T*)z, a, grad, 1.f, stats, 1u, nullptr, nullptr, (T*)dz);
     else hipLaunchKernelGGL((distill_grad_kernel<T, DISTILL_NT, 1>), dim3((unsigned)(n * parts)), dim3(DISTILL_NT), 0, stream, (const T*)z, a, grad, 1.f, stats, (unsigned)parts, nullptr, nullptr, (T*)dz);
     GMK_CHECK_LAUNCH();
@@ -469,6 +472,7 @@ extern "C" int gmk_distill_bwd(const float* grad, const void* z, int ztype, cons
   if (rc != GMK_OK) return rc;
   if (n == 0) return GMK_OK;
   GMK_REQUIRE(grad && z && t && idx && stats && dz, GMK_E_NULL);
+  GMK_REQUIRE(dz != z, GMK_E_UNSUPPORTED);
   GMK_REQUIRE(gmk_aligned_to(z, gmk_dtype_size(ztype)) && gmk_aligned_to(dz, gmk_dtype_size(ztype)) &&
               gmk_aligned_to(t, gmk_dtype_size(ttype)) && gmk_aligned_to(idx, 4) && gmk_aligned_to(labels, 8) &&
               gmk_aligned_to(grad, 4) && gmk_aligned_to(stats, 4), GMK_E_ALIGN);
@@ -483,6 +487,7 @@ extern "C" int gmk_distill_fwd_bwd(const void* z, int ztype, const void* t, int 
   if (rc != GMK_OK) return rc;
   if (n == 0) return GMK_OK;
   GMK_REQUIRE(z && t && idx && loss && dz && (ws || gmk_distill_workspace_bytes(n, C) == 0), GMK_E_NULL);
+  GMK_REQUIRE(dz != z, GMK_E_UNSUPPORTED);
   GMK_REQUIRE(gmk_aligned_to(z, gmk_dtype_size(ztype)) && gmk_aligned_to(dz, gmk_dtype_size(ztype)) &&
               gmk_aligned_to(t, gmk_dtype_size(ttype)) && gmk_aligned_to(idx, 4) && gmk_aligned_to(labels, 8) &&
               gmk_aligned_to(weight, 4) && gmk_aligned_to(loss, 4) && gmk_aligned16(ws), GMK_E_ALIGN);

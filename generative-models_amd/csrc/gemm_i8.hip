@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
   I8Stage<BN, NTHR> sw;
   I8Stage<BM, NTHR> sx;
   const unsigned lds0 = gmk_lds_addr(lds) + __builtin_amdgcn_readfirstlane(wave) * 1024;
-  int l_tile = tile, l_chunk = 0, l_stage = 0;
+  int l_tile = tile, l_chunk = 0, l_stage = 0, l_k = 0;
   auto load_tile = [&]() {
     int m0 = 0, n0 = 0;
     if (l_tile < last) corner(l_tile, m0, n0);
@@ -112,8 +112,8 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
   int l_first = I8Stage<BN, NTHR>::first(0, K);
   auto load = [&](int i) {   // load i of the chunk
     const unsigned to = lds0 + l_stage * BUF;
-    if (i < WLOADS) sw.load(i, to, l_first, l_chunk * I8_BK, K);
-    else sx.load(i - WLOADS, to + BN * I8_BK, l_first, l_chunk * I8_BK, K);
+    if (i < WLOADS) sw.load(i, to, l_first, l_k, K);
+    else sx.load(i - WLOADS, to + BN * I8_BK, l_first, l_k, K);
   };
   auto load_end = [&]() {
     l_stage = l_stage == S - 1 ? 0 : l_stage + 1;
@@ -122,6 +122,7 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
       l_tile += step;
       load_tile();
     }
+    l_k = l_tile < last ? l_chunk * I8_BK : 0;   // a buffer's bytes less this column are what a load is checked against
     // only a last chunk that is not whole, and the one behind it, differ from the chunk before
     if (l_chunk == 0 || (l_chunk + 1) * I8_BK > K) l_first = I8Stage<BN, NTHR>::first(l_chunk * I8_BK, K);
   };

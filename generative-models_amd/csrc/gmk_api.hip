@@ -13,7 +13,7 @@ extern "C" const char* gmk_strerror(int code) {
     case GMK_E_WORKSPACE: return "gmk: workspace too small";
     case GMK_E_NULL: return "gmk: required pointer is NULL";
     case GMK_E_STATE: return "gmk: call out of order (plan recording already active / not active / still recording)";
-    case GMK_E_TOO_LARGE: return "gmk: input exceeds the stated maximum of this allocation-free entry point";
+    case GMK_E_TOO_LARGE: return "gmk: input exceeds the stated maximum of this entry point";
     default: break;
   }
   if (code > 0) return hipGetErrorString((hipError_t)code);

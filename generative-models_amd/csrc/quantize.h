@@ -2,7 +2,6 @@
 #pragma once
 #include "rows.h"
 
-#define GMK_MAX_ROWS 0x7FFFFFFFll   // rows of a launch: one workgroup or wave each, at most 2^31 - 1 workgroups
 
 // The largest magnitude of a row, as the bits of the type without their sign: their order as whole numbers is that of the magnitudes,
 // infinities and NaNs above all.  16-bit types two at a time.

@@ -14,6 +14,9 @@ static inline bool gmk_dtype_ok(int t) { return t == GMK_F32 || t == GMK_BF16 ||
 static inline int gmk_dtype_size(int t) { return t == GMK_F32 ? 4 : 2; }
 static inline bool gmk_aligned_to(const void* p, int size) { return (((uintptr_t)p) & (unsigned)(size - 1)) == 0; }
 
+// A launch has fewer than 2^32 threads.
+static inline bool gmk_grid_ok(int64_t blocks, int threads) { return blocks > 0 && blocks <= 0xFFFFFFFFll / threads; }
+
 // Calls f(T()) with the C++ type of a gmk_dtype (which the caller has checked).
 template <class F>
 static inline auto gmk_with_dtype(int t, F&& f) {

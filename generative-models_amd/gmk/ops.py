@@ -675,8 +675,8 @@ def _distill_args(logits, teacher, index, labels, T, soft, hard):
         _chk_rows("labels", labels, _INT64, (n,), dev)
     elif hard != 0:
         raise ValueError("a hard part needs labels")
-    if not 0 < T < float("inf") or soft - soft != 0 or hard - hard != 0:
-        raise ValueError("the temperature must be finite and above 0, the weights finite")
+    if not 2.0 ** -60 <= T <= 2.0 ** 60 or soft - soft != 0 or hard - hard != 0:
+        raise ValueError("the temperature must lie between 2^-60 and 2^60, the weights must be finite")
     return n, C, k, dev
 
 

@@ -38,7 +38,7 @@ enum gmk_error {
   GMK_E_UNSUPPORTED = -3, /* unsupported option (kernel size, activation, mode) */
   GMK_E_WORKSPACE = -4,   /* workspace too small */
   GMK_E_NULL = -5,        /* required pointer is NULL */
-  GMK_E_TOO_LARGE = -6,   /* input exceeds the stated maximum of an allocation-free (static scratch) entry point */
+  GMK_E_TOO_LARGE = -6,   /* input exceeds the stated maximum of an entry point */
   GMK_E_STATE = -7        /* call out of order: gmk_plan_begin while recording, gmk_plan_mark / _end while not, replay of a plan still being recorded */
 };
 
@@ -330,7 +330,7 @@ enum gmk_dtype { GMK_F32 = 0, GMK_BF16 = 1, GMK_F16 = 2 };
 
 /* gmk_quantize_rows: x (M,K) -> q (M,ldq) int8, scale (M) fp32, one scale for each row:
  *   scale = max(fl32(max_k |x| / 127), 2^-126), q = the whole number nearest x / scale (halves to even; exact, whatever the
- *   quotient's own rounding), zeros in columns [K, ldq).  ldq >= K, ldq % 16 == 0.  A row that holds an infinity or a NaN
+ *   quotient's own rounding), zeros in columns [K, ldq).  K <= ldq <= 2^30, ldq % 16 == 0.  A row that holds an infinity or a NaN
  *   gets zeros and a NaN scale, so that whatever is made of it is NaN. */
 int gmk_quantize_rows(const void* x, int xtype, signed char* q, float* scale, int64_t M, int K, int ldq,
                       gmk_stream_t stream);
@@ -364,14 +364,17 @@ int gmk_topk_rows(const void* x, int xtype, void* value, int* index, int64_t n, 
  *     d loss / d z_c = soft T (q_c - p_c) + hard (softmax(z)_c - [c = label]).
  *   An idx outside [0, C) is no entry, and a row without an entry of a weight above 0 has no soft part; a label outside [0, C)
  *   (say -100) or labels == NULL: no hard part.  A row whose logits are all -inf gives loss 0 and gradient 0.  The same class may be
- *   listed more than once.  z and dz share ztype, t has ttype.  1 <= k <= GMK_DISTILL_MAX_K, C < 2^31, T > 0.
+ *   listed more than once.  z and dz share ztype, t has ttype.  1 <= k <= GMK_DISTILL_MAX_K, C < 2^31, T between 2^-60 and 2^60.
  * gmk_distill_fwd: loss (n) fp32 and stats (n,3) fp32 (the row's maximum and its two sums of exponentials) for the backward pass.
- * gmk_distill_bwd: dz (n,C) = grad[row] * d loss / d z, grad (n) fp32.  Rows with grad 0 give 0 (nothing of them is read).
+ * gmk_distill_bwd: dz (n,C) = grad[row] * d loss / d z, grad (n) fp32; everything else as in the forward call.  Rows with grad 0 give
+ *   0 (nothing of them is read).
  * gmk_distill_fwd_bwd: both in one call, each logit read from memory once where a row fits the registers of a workgroup:
  *   loss[row] = weight[row] * loss, dz = scale * weight[row] * d loss / d z; weight (n) fp32, or NULL for ones.  Rows with
  *   weight 0 (padding) give 0 and 0 whatever they hold.
  *   ws >= gmk_distill_workspace_bytes(n, C) bytes (0: NULL is fine), the same for all three. */
 #define GMK_DISTILL_MAX_K 256
+#define GMK_DISTILL_MIN_T 0x1p-60f
+#define GMK_DISTILL_MAX_T 0x1p60f
 size_t gmk_distill_workspace_bytes(int64_t n, int64_t C);
 int gmk_distill_fwd(const void* z, int ztype, const void* t, int ttype, const int* idx, const int64_t* labels, float* loss,
                     float* stats, int64_t n, int64_t C, int k, float T, float soft, float hard, void* ws, size_t ws_bytes,

@@ -290,6 +290,46 @@ def test_teacher_to_student_run():
     _all_forms(student, value.cpu(), index.cpu(), labels, 2.0, 0.9, 0.1)
 
 
+@gpu
+def test_operators_in_a_launch_plan():
+    """Recorded once and replayed from C on other inputs by pointer substitution: the same bits as direct calls."""
+    import ctypes as C
+    from gmk import lib, check, ops
+    h = lib()
+    B, F, classes, k = 40, 300, 50, 6
+    w = ops.quantize_rows(_randn(1, classes, F).cuda())
+    labels = torch.randint(0, classes, (B,), generator=torch.Generator().manual_seed(2)).cuda()
+    student = [_randn(10 + i, B, classes).cuda() for i in range(3)]
+    x = [_randn(20 + i, B, F).cuda() for i in range(3)]
+
+    def step(x, student):
+        value, index = ops.topk_rows(ops.linear_i8(x, *w), k)
+        loss, stats = ops.distill_fwd(student, value, index, labels, 2.0, 0.5, 0.5)
+        q, s = ops.quantize_rows(x)
+        return [value, index, loss, stats, ops.distill_bwd(loss, student, value, index, labels, stats, 2.0, 0.5, 0.5), q, s, ops.matmul_i8(q, s, *w),
+                *ops.distill_fwd_bwd(student, value, index, labels, 2.0, 0.5, 0.5)]
+
+    want = [[t.clone() for t in step(x[i], student[i])] for i in range(3)]
+    plan = C.c_void_p()
+    keep = ops._rec_keep = []
+    check(h.gmk_plan_begin(C.byref(plan)))
+    try:
+        out = step(x[0], student[0])
+    finally:
+        check(h.gmk_plan_end())
+        ops._rec_keep = None
+    assert h.gmk_plan_calls(plan) == 7
+    src = (C.c_void_p * 2)(x[0].data_ptr(), student[0].data_ptr())
+    nb = (C.c_size_t * 2)(x[0].numel() * 4, student[0].numel() * 4)
+    for i in (1, 2, 0):
+        dst = (C.c_void_p * 2)(x[i].data_ptr(), student[i].data_ptr())
+        check(h.gmk_train_step_enqueue(plan, 0, h.gmk_plan_segments(plan), 2, src, dst, nb))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+    h.gmk_plan_destroy(plan)
+    assert len(keep) > 7
+
+
 # ---------------------------------------------------------------- refusals (no GPU)
 
 def test_distill_c_entries_refuse_bad_arguments():
@@ -303,21 +343,23 @@ def test_distill_c_entries_refuse_bad_arguments():
         return h.gmk_distill_fwd(c["z"], c["zt"], c["t"], c["tt"], c["idx"], c["lab"], c["loss"], c["st"], c["n"], c["C"], c["k"], c["T"], c["s"], c["h"], c["w"], c["wb"], None)
 
     def bwd(**c):
-        c = {**base, "g": p, "st": p, "dz": p, **c}
+        c = {**base, "g": p, "st": p, "dz": ctypes.c_void_p(1 << 20), **c}
         return h.gmk_distill_bwd(c["g"], c["z"], c["zt"], c["t"], c["tt"], c["idx"], c["lab"], c["st"], c["dz"], c["n"], c["C"], c["k"], c["T"], c["s"], c["h"], None)
 
     def both(**c):
-        c = {**base, "wt": None, "loss": p, "dz": p, "sc": 1.0, "w": p, "wb": 1 << 40, **c}
+        c = {**base, "wt": None, "loss": p, "dz": ctypes.c_void_p(1 << 20), "sc": 1.0, "w": p, "wb": 1 << 40, **c}
         return h.gmk_distill_fwd_bwd(c["z"], c["zt"], c["t"], c["tt"], c["idx"], c["lab"], c["wt"], c["loss"], c["dz"], c["n"], c["C"], c["k"], c["T"], c["s"], c["h"], c["sc"], c["w"], c["wb"], None)
 
     for f in (fwd, bwd, both):
-        assert f(zt=3) == f(tt=-1) == f(T=0.0) == f(T=-1.0) == f(T=nan) == f(T=float("inf")) == f(s=nan) == f(h=float("inf")) == -3
+        assert f(zt=3) == f(tt=-1) == f(T=0.0) == f(T=1e-20) == f(T=1e20) == f(T=-1.0) == f(T=nan) == f(T=float("inf")) == f(s=nan) == f(h=float("inf")) == -3
         assert f(n=-1) == f(C=0) == f(k=0) == -1
         assert f(k=257) == f(C=1 << 31) == -6
         assert f(z=None) == f(t=None) == f(idx=None) == -5
         assert f(z=odd) == f(t=odd) == f(idx=odd) == f(lab=ctypes.c_void_p(4100)) == -2
         assert f(n=0, z=None) == 0
     assert fwd(loss=None) == fwd(st=None) == bwd(g=None) == bwd(st=None) == bwd(dz=None) == both(loss=None) == both(dz=None) == -5
+    other = ctypes.c_void_p(8192)
+    assert bwd(z=other, dz=other) == both(z=other, dz=other) == -3
     assert both(wt=odd) == both(dz=odd) == both(loss=odd) == bwd(g=odd) == fwd(st=odd) == -2
     need = int(h.gmk_distill_workspace_bytes(2, 1 << 20))
     assert need == 0 or fwd(C=1 << 20, wb=need - 1) == both(C=1 << 20, wb=need - 1) == -4
@@ -327,6 +369,20 @@ def test_distill_wrappers_refuse_cpu_tensors():
     from gmk import ops
     z, t, i = torch.zeros(2, 5), torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.int32)
     for call in (lambda: ops.distill_fwd(z, t, i), lambda: ops.distill_fwd_bwd(z, t, i), lambda: ops.distill_bwd(torch.ones(2), z, t, i, None, torch.ones(2, 3))):
+        with pytest.raises(ValueError):
+            call()
+
+
+@gpu
+def test_operators_refuse_another_device(monkeypatch):
+    """Tensors that are not on the current device, whose stream the launch would go to."""
+    from gmk import ops
+    x = torch.randn(4, 32, device="cuda")
+    q, s = ops.quantize_rows(x)
+    v, i = ops.topk_rows(x, 3)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    for call in (lambda: ops.quantize_rows(x), lambda: ops.linear_i8(x, q, s), lambda: ops.matmul_i8(q, s, q, s), lambda: ops.topk_rows(x, 3), lambda: ops.distill_fwd(x, v, i),
+                 lambda: ops.distill_fwd_bwd(x, v, i)):
         with pytest.raises(ValueError):
             call()
 

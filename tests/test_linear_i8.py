@@ -274,6 +274,7 @@ def test_c_entries_refuse_bad_arguments():
     assert q(M=-1) == q(K=0) == q(ld=16) == q(ld=24) == E["shape"]
     assert q(x=None) == q(q=None) == q(s=None) == E["null"]
     assert q(x=odd) == q(q=ctypes.c_void_p(4100)) == q(s=odd) == E["align"]
+    assert q(K=1 << 30, ld=(1 << 30) + 16) == q(M=1 << 40) == E["large"]
     assert q(M=0, x=None) == 0
     g = lambda **k: h.gmk_gemm_i8(*{**dict(xq=p, xs=p, wq=p, ws=p, b=None, y=p, yt=0, M=2, K=32, N=3, act=0, st=None), **k}.values())  # noqa: E731
     assert g(yt=9) == g(act=9) == g(act=-1) == E["unsupported"]
