@@ -289,18 +289,22 @@ __global__ __launch_bounds__(DISTILL_NT) void distill_part_kernel(const T* __res
   }
 }
 
-// a row's maximum and sums from its parts', in every thread (a fixed order: every workgroup of the row gets the same)
+// a row's maximum and sums from its parts', in every thread (a fixed order: every workgroup of the row gets the same); `mine`: those of part
+// threadIdx.x, loaded before
 template <int NT>
-__device__ __forceinline__ DistillStats distill_join(const DistillArgs& a, const float* __restrict__ part, unsigned parts, float* red) {
-  DistillStats s = {-__builtin_inff(), 0.f, 0.f};
-  for (unsigned i = threadIdx.x; i < parts; i += NT) s.mx = __builtin_elementwise_maximum(s.mx, part[3 * (int64_t)i]);
+__device__ __forceinline__ DistillStats distill_join(const DistillArgs& a, const DistillStats& mine, const float* __restrict__ part, unsigned parts, float* red) {
+  DistillStats s = {mine.mx, 0.f, 0.f};
+  for (unsigned i = threadIdx.x + NT; i < parts; i += NT) s.mx = __builtin_elementwise_maximum(s.mx, part[3 * (int64_t)i]);
   s.mx = gmk_block_maximum_all<NT>(s.mx, red);
-  if (s.mx != -__builtin_inff())
-    for (unsigned i = threadIdx.x; i < parts; i += NT) {
+  if (s.mx != -__builtin_inff()) {
+    s.st = mine.st * distill_exp2((mine.mx - s.mx) * a.at);
+    s.s1 = mine.s1 * distill_exp2((mine.mx - s.mx) * a.a1);
+    for (unsigned i = threadIdx.x + NT; i < parts; i += NT) {
       const float d = part[3 * (int64_t)i] - s.mx;
       s.st += part[3 * (int64_t)i + 1] * distill_exp2(d * a.at);
       s.s1 += part[3 * (int64_t)i + 2] * distill_exp2(d * a.a1);
     }
+  }
   gmk_block_sum2_all<NT>(s.st, s.s1, red);
   if (a.same) s.s1 = s.st;
   return s;
@@ -334,16 +338,20 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(const T* __restrict__ 
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) keep[i] = gmk_row_piece(zr, e0 + i * NT * VEC, a.C);
   }
+  DistillStats s = {-__builtin_inff(), 0.f, 0.f};
+  if (MODE != 1 && threadIdx.x < parts) {
+    const float* p = from_parts + (row * parts + threadIdx.x) * 3;
+    s = {p[0], p[1], p[2]};
+  }
   if (threadIdx.x < 64) {
     const bool has = distill_entries(a, zr, row, en);
     if (threadIdx.x == 0) s_has = has;
   }
-  DistillStats s;
   if constexpr (MODE == 1) {
     s = {from_parts[row * 3], from_parts[row * 3 + 1], from_parts[row * 3 + 2]};
     __syncthreads();
   } else {
-    s = distill_join<NT>(a, from_parts + row * parts * 3, parts, red);
+    s = distill_join<NT>(a, s, from_parts + row * parts * 3, parts, red);
     if (NT == 64) __syncthreads();
   }
   const bool has = s_has;
@@ -373,12 +381,12 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(const T* __restrict__ 
 
 static int64_t distill_parts(int64_t C, int vec) { return (C + DISTILL_NT * DISTILL_KEEP * vec - 1) / (DISTILL_NT * DISTILL_KEEP * vec); }
 
-// Rows in parts: those that no workgroup's registers hold (8 pieces for each of 1024 threads), and many rows that would leave too much of
-// such a workgroup idle: 2048x50000 bf16 151 us, whole rows 170; but 2048x65536 189 and 174, 128x20000 fp32 12.7 and 12.1.  The loss alone
-// reads a part once either way: 2048x65536 76 us in parts, whole rows 107 (one workgroup of 1024 threads a unit at a time).
+// Rows in parts: those that no workgroup's registers hold (8 pieces for each of 1024 threads), and, for the loss alone, many that only a
+// workgroup of 1024 threads would: 2048x65536 bf16 76 us in parts, whole rows 107.  With the gradient whole rows win, as they are read
+// once: 511 rows of 49000 32.8 us, 512 in parts 40.0.
 static bool distill_in_parts(int mode, int64_t n, int64_t C, int vec) {
   const int64_t pieces = (C + vec - 1) / vec;
-  return pieces > 8192 || (n >= 512 && pieces > 4096 && (mode == 0 || pieces <= 7168));
+  return pieces > 8192 || (mode == 0 && n >= 512 && pieces > 4096);
 }
 
 extern "C" size_t gmk_distill_workspace_bytes(int64_t n, int64_t C) {
@@ -427,11 +435,20 @@ static int distill_launch(const void* z, int ztype, const DistillArgs& a, const 
       return GMK_OK;
     };
     const int64_t pieces = (a.C + VEC - 1) / VEC;
+    // As few pieces a thread as hold the row (one that no thread has costs what the others do: 4096x20000 bf16 73 us with 5 of 512 threads,
+    // 106 with 8), and as few threads, so that several workgroups of a unit are at different steps.
     if (pieces <= 64) return go(distill_row_kernel<T, 64, 1, MODE>, 64);
+    if (pieces <= 128) return go(distill_row_kernel<T, 64, 2, MODE>, 64);
     if (pieces <= 256) return go(distill_row_kernel<T, 64, 4, MODE>, 64);
+    if (pieces <= 512) return go(distill_row_kernel<T, 256, 2, MODE>, 256);
     if (pieces <= 1024) return go(distill_row_kernel<T, 256, 4, MODE>, 256);
+    if (pieces <= 1536) return go(distill_row_kernel<T, 256, 6, MODE>, 256);
     if (pieces <= 2048) return go(distill_row_kernel<T, 256, 8, MODE>, 256);
+    if (pieces <= 2560) return go(distill_row_kernel<T, 256, 10, MODE>, 256);
+    if (pieces <= 3072) return go(distill_row_kernel<T, 512, 6, MODE>, 512);
+    if (pieces <= 3584) return go(distill_row_kernel<T, 512, 7, MODE>, 512);
     if (pieces <= 4096) return go(distill_row_kernel<T, 512, 8, MODE>, 512);
+    if (pieces <= 6144) return go(distill_row_kernel<T, 1024, 6, MODE>, 1024);
     return go(distill_row_kernel<T, 1024, 8, MODE>, 1024);
   });
 }

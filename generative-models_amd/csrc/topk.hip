@@ -30,8 +30,8 @@ __device__ __forceinline__ unsigned topk_index(u64 pair) { return 0xFFFFFFFFu - 
 #define TOPK_NT 256      // threads of a workgroup, or 64 where rows are short and many
 #define TOPK_CAND(nt) ((nt) == 64 ? 512 : 1024)   // elements that are collected at most
 #define TOPK_PAD 16      // and zeros behind them, which are below every pair
-#define TOPK_SEGS 8      // segments of a thread: 16 take LDS from two of the 8 workgroups that a compute unit holds
 #define TOPK_LOADS 4     // pieces of 16 bytes that a thread loads at once
+#define TOPK_SEGS 8      // segments of a thread: 16 take LDS from two of the 8 workgroups that a compute unit holds
 
 #define TOPK_WAVE 4096       // elements of a row that one wave takes at most
 #define TOPK_PART 4096       // elements of a part at least
@@ -139,13 +139,13 @@ __device__ __forceinline__ void topk_row(const T* __restrict__ x, int64_t C, uns
 #pragma unroll
   for (int i = 0; i < MX; ++i) best[i] = low;
   const int64_t e0 = (int64_t)tid * VEC;
+  gmk_u32x4 v[TOPK_LOADS];   // behind the loop: the last round, which is all of a short row
   for (int64_t g = 0, s = 0; g < groups; g += per_seg, ++s) {
     float mine[MX];
 #pragma unroll
     for (int i = 0; i < MX; ++i) mine[i] = low;
     const int64_t end = g + per_seg < groups ? g + per_seg : groups;
     for (int64_t h = g; h < end; ++h) {
-      gmk_u32x4 v[TOPK_LOADS];
       const int64_t e = e0 + h * GROUP;
       if ((h + 1) * GROUP <= C) {
 #pragma unroll
@@ -197,16 +197,21 @@ __device__ __forceinline__ void topk_row(const T* __restrict__ x, int64_t C, uns
       }
     }
   };
-  for (int64_t g = 0, s = 0; g < groups; g += per_seg, ++s) {
-    if (sh.seg[s][tid] < limit) continue;
-    const int64_t end = g + per_seg < groups ? g + per_seg : groups;
-    for (int64_t h = g; h < end; ++h) {
-      gmk_u32x4 v[TOPK_LOADS];
-      const int64_t e = e0 + h * GROUP;
+  if (groups == 1) {
 #pragma unroll
-      for (int i = 0; i < TOPK_LOADS; ++i) v[i] = gmk_row_piece(x, e + i * LOAD, C);
+    for (int i = 0; i < TOPK_LOADS; ++i) collect(v[i], e0 + i * LOAD);
+  } else {
+    for (int64_t g = 0, s = 0; g < groups; g += per_seg, ++s) {
+      if (sh.seg[s][tid] < limit) continue;
+      const int64_t end = g + per_seg < groups ? g + per_seg : groups;
+      for (int64_t h = g; h < end; ++h) {
+        gmk_u32x4 v[TOPK_LOADS];
+        const int64_t e = e0 + h * GROUP;
 #pragma unroll
-      for (int i = 0; i < TOPK_LOADS; ++i) collect(v[i], e + i * LOAD);
+        for (int i = 0; i < TOPK_LOADS; ++i) v[i] = gmk_row_piece(x, e + i * LOAD, C);
+#pragma unroll
+        for (int i = 0; i < TOPK_LOADS; ++i) collect(v[i], e + i * LOAD);
+      }
     }
   }
   __syncthreads();

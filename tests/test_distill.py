@@ -114,7 +114,7 @@ def _all_forms(z, t, idx, labels, T, soft, hard, weight=None, scale=0.37):
 
 
 SHAPES = [(1, 1, 1), (2, 2, 2), (256, 10, 3), (7, 10, 10), (300, 37, 5), (5, 64, 8), (3, 127, 64), (64, 1000, 10), (9, 2049, 100), (5, 4096, 256), (33, 8191, 20), (6, 10007, 20),
-          (3, 16384, 64), (2, 32768, 64), (3, 40001, 30), (2, 65536, 128), (1, 70001, 256), (2, 131073, 64), (3, 200003, 50)]
+          (3, 16384, 64), (2, 32768, 64), (3, 40001, 30), (2, 65536, 128), (1, 70001, 256), (2, 131073, 64), (3, 200003, 50), (520, 34000, 3), (1, 1200001, 200)]
 
 
 @gpu
