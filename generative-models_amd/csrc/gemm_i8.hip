@@ -436,6 +436,7 @@ template <class T, class X, int NT>
 static int gemm_i8_rows_launch(const X* x, const float* xscale, const signed char* wq, const float* wscale, const float* bias, T* y, int M,
                                int K, int N, int act, int Kx, hipStream_t stream) {
   const int64_t tm = (M + 15) / 16, tn = (N + NT * 16 - 1) / (NT * 16);
+  GMK_REQUIRE(gmk_grid_ok(tm * tn, 512), GMK_E_TOO_LARGE);
   const int bytes = std::is_same<X, signed char>::value ? 0 : M * K;
   hipLaunchKernelGGL((gemm_i8_rows_kernel<T, X, NT, 8, 4>), dim3((unsigned)(tm * tn)), dim3(512), bytes, stream, x, xscale, wq, wscale, bias, y, M,
                      K, N, act, (int)tm, Kx);
@@ -446,7 +447,7 @@ static int gemm_i8_rows_launch(const X* x, const float* xscale, const signed cha
 static int gemm_i8_check(int M, int K, int N, int ytype, int act) {
   GMK_REQUIRE(gmk_dtype_ok(ytype) && act >= GMK_ACT_NONE && act <= GMK_ACT_SIGMOID, GMK_E_UNSUPPORTED);
   GMK_REQUIRE(M >= 0 && N > 0 && K > 0, GMK_E_SHAPE);
-  GMK_REQUIRE(K <= GMK_I8_MAX_K, GMK_E_TOO_LARGE);
+  GMK_REQUIRE(K <= GMK_I8_MAX_K && M <= GMK_I8_MAX_ROWS && N <= GMK_I8_MAX_ROWS, GMK_E_TOO_LARGE);   // rows and tiles are counted in 32 bits
   return GMK_OK;
 }
 

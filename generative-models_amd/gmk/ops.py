@@ -1,7 +1,8 @@
 """Tensor-level wrappers over the C ABI (no autograd here: the autograd.Functions live in models/autoencoders.py).
 
 Every function takes contiguous fp32 CUDA tensors, allocates its outputs with torch (device
-memory plumbing), and launches on torch's current stream.
+memory plumbing), and launches on torch's current stream.  The functions behind "a classifier made smaller" take bf16 and
+fp16 too.
 """
 import functools
 import os

@@ -9,12 +9,13 @@
  *   - plain pointers + sizes; every buffer (inputs, outputs, workspace) is DEVICE memory owned by
  *     the caller; the library never allocates, frees or retains a pointer;
  *   - tensors are fp32, contiguous, NCHW (activations), OIHW (conv weights), IOHW (transposed-conv
- *     weights), [out][in] (linear weights): the layouts of the reference's state_dict;
+ *     weights), [out][in] (linear weights): the layouts of the reference's state_dict (the last section, "a classifier made
+ *     smaller", names its own types);
  *   - asynchronous launch on `stream` (a hipStream_t passed as void*; NULL = default stream), no internal
  *     synchronisation, re-entrant across streams and devices.  State the library keeps, all of it listed here: (1) the
  *     per-device kernel-path selection of gmk_conv_set_thin_paths (one atomic word per device); (2) per-device caches that
  *     only ever grow (event ring of gmk_stream_wait_stream, raised dynamic-LDS limits, the address of the static scratch of
- *     gmk_vae_loss_fwd_bwd_static); (3) the calling thread's plan being recorded between gmk_plan_begin / gmk_plan_end;
+ *     gmk_vae_loss_fwd_bwd_static, the number of compute units); (3) the calling thread's plan being recorded between gmk_plan_begin / gmk_plan_end;
  *     (4) profiling knobs read once from the environment (GMK_WINO, GMK_EVENT_SCOPE, GMK_*_DBG: ablation builds, 0 in production);
  *   - return 0 on success, a negative GMK_E_* on a rejected argument, a positive hipError_t if a
  *     launch failed; gmk_strerror() names either.
@@ -84,7 +85,8 @@ int gmk_conv_get_thin_paths(int* thin_in, int* thin_outv);
  * one from Python + ctypes they cost 0.8 ms of host time against 1.0 ms of GPU time at batch 256.  A plan records them
  * once and replays them from C:
  * gmk_plan_begin(&plan): from now until gmk_plan_end(), every launching entry point of this header called on THIS host
- *   thread (conv / deconv / linear / loss / reparam / pool / upsample / ew_mul / gmk_stream_wait_stream) runs as usual and
+ *   thread (conv / deconv / linear / loss / reparam / pool / upsample / ew_mul / gmk_stream_wait_stream,
+ *   quantize_rows / gemm_i8 / linear_i8 / topk_rows / distill) runs as usual and
  *   is also appended to the plan: its own address and its arguments by value.  One recording per thread at a time.
  * gmk_plan_mark(): closes the current segment and returns its index (>= 0): the host side marks the points where it has
  *   work of its own between launches (a gradient bucket's all-reduce).  gmk_plan_end() closes the last segment.
@@ -325,7 +327,7 @@ int gmk_softmax_stats(const float* logits, int64_t n, int C, int topn, float eps
  * Floating tensors are fp32, bf16 or fp16 (gmk_dtype), row-major and contiguous, aligned to their element; every sum, maximum and
  * scale is held in 32 bits or more, and values are rounded to the output's type once.  Calls with zero rows launch nothing and
  * return 0.  8-bit buffers and workspaces are 16-byte aligned; outputs overlap no input.  Results do not depend on the launch's
- * timing (no float atomics). */
+ * timing (no float atomics).  Up to 2^24 - 1 rows are always taken; a launch that would have 2^32 threads is GMK_E_TOO_LARGE. */
 enum gmk_dtype { GMK_F32 = 0, GMK_BF16 = 1, GMK_F16 = 2 };
 
 /* gmk_quantize_rows: x (M,K) -> q (M,ldq) int8, scale (M) fp32, one scale for each row:
@@ -336,9 +338,10 @@ int gmk_quantize_rows(const void* x, int xtype, signed char* q, float* scale, in
                       gmk_stream_t stream);
 
 /* gmk_gemm_i8: y (M,N) = act((sum_k xq[m][k] wq[n][k]) * xscale[m] * wscale[n] + bias[n]), the sum exact in 32-bit
- *   integers.  xq (M,K), wq (N,K) int8 in [-128, 127], K % 16 == 0 (rows that gmk_quantize_rows padded are whole), K <= GMK_I8_MAX_K;
- *   bias (N) fp32 or NULL; act: enum gmk_act. */
+ *   integers.  xq (M,K), wq (N,K) int8 in [-128, 127], K % 16 == 0 (rows that gmk_quantize_rows padded are whole), K <= GMK_I8_MAX_K,
+ *   M and N <= GMK_I8_MAX_ROWS; bias (N) fp32 or NULL; act: enum gmk_act. */
 #define GMK_I8_MAX_K 131056
+#define GMK_I8_MAX_ROWS (1 << 30) /* M and N */
 int gmk_gemm_i8(const signed char* xq, const float* xscale, const signed char* wq, const float* wscale, const float* bias,
                 void* y, int ytype, int M, int K, int N, int act, gmk_stream_t stream);
 /* gmk_linear_i8_fwd: the same from floating activations: x (M,K) is quantised row by row as gmk_quantize_rows does, and
@@ -364,7 +367,8 @@ int gmk_topk_rows(const void* x, int xtype, void* value, int* index, int64_t n, 
  *     d loss / d z_c = soft T (q_c - p_c) + hard (softmax(z)_c - [c = label]).
  *   An idx outside [0, C) is no entry, and a row without an entry of a weight above 0 has no soft part; a label outside [0, C)
  *   (say -100) or labels == NULL: no hard part.  A row whose logits are all -inf gives loss 0 and gradient 0.  The same class may be
- *   listed more than once.  z and dz share ztype, t has ttype.  1 <= k <= GMK_DISTILL_MAX_K, C < 2^31, T between 2^-60 and 2^60.
+ *   listed more than once.  The soft loss is a difference of sums in 32 bits, known to about soft T^2 2^-20: at temperatures far above the
+ *   logits' differences it loses its digits (the gradient does not).  z and dz share ztype, t has ttype.  1 <= k <= GMK_DISTILL_MAX_K, C < 2^31, T between 2^-60 and 2^60.
  * gmk_distill_fwd: loss (n) fp32 and stats (n,3) fp32 (the row's maximum and its two sums of exponentials) for the backward pass.
  * gmk_distill_bwd: dz (n,C) = grad[row] * d loss / d z, grad (n) fp32; everything else as in the forward call.  Rows with grad 0 give
  *   0 (nothing of them is read).

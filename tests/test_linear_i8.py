@@ -279,14 +279,14 @@ def test_c_entries_refuse_bad_arguments():
     g = lambda **k: h.gmk_gemm_i8(*{**dict(xq=p, xs=p, wq=p, ws=p, b=None, y=p, yt=0, M=2, K=32, N=3, act=0, st=None), **k}.values())  # noqa: E731
     assert g(yt=9) == g(act=9) == g(act=-1) == E["unsupported"]
     assert g(M=-1) == g(K=0) == g(K=20) == g(N=0) == E["shape"]
-    assert g(K=131072) == E["large"]
+    assert g(K=131072) == g(M=(1 << 31) - 1) == g(N=(1 << 30) + 1) == g(M=1, K=16, N=1 << 28) == E["large"]
     assert g(xq=None) == g(xs=None) == g(wq=None) == g(ws=None) == g(y=None) == E["null"]
     assert g(xq=ctypes.c_void_p(4104)) == g(wq=ctypes.c_void_p(4104)) == g(b=odd) == g(y=odd) == E["align"]
     assert g(M=0) == 0
     f = lambda **k: h.gmk_linear_i8_fwd(*{**dict(x=p, xt=0, wq=p, ws=p, b=None, y=p, yt=0, M=20, K=20, N=3, act=0, w=p, wb=1 << 40, st=None), **k}.values())  # noqa: E731
     assert f(xt=5) == f(yt=5) == f(act=12) == E["unsupported"]
     assert f(M=-2) == f(K=-1) == f(N=0) == E["shape"]
-    assert f(K=131057) == E["large"]
+    assert f(K=131057) == f(M=(1 << 31) - 1) == f(N=(1 << 31) - 1) == f(M=1, N=1 << 28) == E["large"]
     assert f(x=None) == f(w=None) == f(y=None) == E["null"]
     assert f(x=odd) == f(w=ctypes.c_void_p(4104)) == E["align"]
     assert f(wb=int(h.gmk_linear_i8_workspace_bytes(20, 20, 3)) - 1) == E["workspace"]
