@@ -6,6 +6,7 @@
 // kernel selection, same launches.
 #pragma once
 #include <stddef.h>
+#include <hip/hip_runtime.h>
 #include <functional>
 
 namespace gmk_plan_detail {
@@ -29,15 +30,22 @@ void push(std::function<int(const Subst&)> call);
 template <class T> inline T sub(const Subst&, T v) { return v; }
 template <class T> inline T* sub(const Subst& s, T* v) { return (T*)s.map((const void*)v); }
 
+// false: no host memory for the call's record (an exception must not leave the C entry point that records)
 template <class... A, class... B>
-inline void record(int (*fn)(A...), B... args) {
+inline bool record(int (*fn)(A...), B... args) {
   static_assert(sizeof...(A) == sizeof...(B), "hook must pass every argument of the entry point");
-  push([=](const Subst& s) { return fn(sub(s, static_cast<A>(args))...); });
+  try {
+    push([=](const Subst& s) { return fn(sub(s, static_cast<A>(args))...); });
+    return true;
+  } catch (...) {
+    return false;
+  }
 }
 
 }  // namespace gmk_plan_detail
 
 #define GMK_PLAN_HOOK(fn, ...)                                                        \
   do {                                                                                \
-    if (gmk_plan_detail::recording()) gmk_plan_detail::record(&fn, __VA_ARGS__);      \
+    if (gmk_plan_detail::recording() && !gmk_plan_detail::record(&fn, __VA_ARGS__))   \
+      return (int)hipErrorOutOfMemory;                                                \
   } while (0)
