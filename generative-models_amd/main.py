@@ -156,6 +156,8 @@ def main(args):
             teacher = None
             if args.teacher_checkpoint is not None:
                 teacher = torch.load(args.teacher_checkpoint, map_location=device, weights_only=False)
+                if isinstance(teacher, dict):
+                    raise NotImplementedError('\n\nteacher checkpoint must be a full saved model, not a state_dict\n\n')
                 teacher.int8_fc = args.teacher_int8
             classifier = train_classifier(args, classifier=None, train_dataloader=train_dataloader,
                                           test_dataloader=test_dataloader, device=device, teacher=teacher)

@@ -67,7 +67,8 @@ class Classifier(nn.Module):
                 for layer in (self.fc, self.fc_out):
                     w, b = out[layer]
                     out[layer] = (*ops.quantize_rows(w), b)
-        self.__dict__["_gmk_fold"] = (key, out)
+        # the tensors themselves are kept too: memory that a later weight could be given is no key
+        self.__dict__["_gmk_fold"] = (key, out, [t.detach() for t in tensors])
         return out
 
     def _forward_gmk(self, x):
@@ -131,7 +132,8 @@ class _DistillFn(torch.autograd.Function):
 def distillation_loss(outputs, value, index, labels=None, T=4.0, soft=0.9, hard=0.1):
     """Loss of each sample (n,) of a student's logits (n, C): soft T^2 KL(teacher || student) at temperature T over the teacher's kept logits
     `value` (n, k) of the classes `index` (n, k) int32 (gmk.ops.topk_rows; -1: no entry), plus hard * cross entropy where labels (n,) are
-    given (outside [0, C): none).  CUDA tensors; outputs fp32, bf16 or fp16, under autograd."""
+    given (outside [0, C): none).  CUDA tensors; outputs fp32, bf16 or fp16, under autograd.  In 32 bits the soft part is known to about
+    soft T^2 2^-20, so that it loses its digits at temperatures far above the logits' differences; the gradient keeps them."""
     if labels is None:
         hard = 0.0
     return _DistillFn.apply(outputs.contiguous(), value.detach(), index, labels, float(T), float(soft), float(hard))

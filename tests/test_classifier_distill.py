@@ -66,6 +66,25 @@ def test_int8_classifier_layers(monkeypatch, batch):
 
 
 @gpu
+def test_int8_layers_follow_replaced_weights():
+    """A weight whose storage is exchanged twice between two calls, the second time for memory that the first one left: the answers are
+    those of a classifier that never saw the others."""
+    m, _ = _classifier()
+    m = m.cuda().eval()
+    m.int8_fc = True
+    x = torch.rand(8, 3, 32, 32, generator=torch.Generator().manual_seed(5)).cuda()
+    m.fc.weight.data = _randn(1, *m.fc.weight.shape).cuda() / 64
+    m(x)
+    for seed in (2, 3):
+        m.fc.weight.data = _randn(seed, *m.fc.weight.shape).cuda() / 64
+    fresh, _ = _classifier()
+    fresh = fresh.cuda().eval()
+    fresh.load_state_dict(m.state_dict())
+    fresh.int8_fc = True
+    assert torch.equal(m(x), fresh(x))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_distillation_loss_gradient(dtype):
     """The gradient through autograd, with different weights of the samples, against automatic differentiation in 64 bits."""
