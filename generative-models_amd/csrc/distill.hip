@@ -8,11 +8,10 @@
 // The maximum is subtracted before anything is scaled: rows of the type's lowest value give 0 and not inf - inf.
 //
 // A row that the registers of a workgroup hold is read once: maximum, sums and gradient from there (distill_row_kernel).  Longer rows, and
-// few rows, are taken in parts: the parts' maxima and sums (distill_part_kernel), then everything else, each part's workgroup joining them
+// many long ones for the loss alone, are taken in parts: the parts' maxima and sums (distill_part_kernel), then everything else, each part's workgroup joining them
 // again (distill_grad_kernel, which is the backward pass too).  The gradient of the listed classes is written over what the dense pass
 // wrote, by the workgroup that wrote it.
 #include "rows.h"
-#include "quantize.h"
 #include "plan.h"
 
 struct DistillArgs {
@@ -98,13 +97,6 @@ struct DistillGrad {
     c1 = en.label >= 0 && !empty ? g * a.hard : 0.f;
     gt = ct != 0.f ? ct / s.st : 0.f;
     g1 = c1 != 0.f ? c1 / s.s1 : 0.f;
-  }
-  __device__ __forceinline__ float dense(const DistillArgs& a, float z) const {
-    const float d = z - mx;
-    float r = 0.f;
-    if (gt != 0.f) r = distill_exp2(d * a.at) * gt;
-    if (g1 != 0.f) r = fmaf(distill_exp2(d * a.a1), g1, r);
-    return r;
   }
   // VEC values of a piece
   template <class T>
@@ -215,6 +207,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(const T* __restrict__ z
     const bool has = distill_entries(a, zr, row, en);
     if (threadIdx.x == 0) s_has = has;
   }
+  if (NT == 64) __syncthreads();   // the reductions of a single wave have no barrier
   DistillStats s = {-__builtin_inff(), 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) s.mx = distill_most<T>(keep[i], s.mx);
@@ -437,18 +430,18 @@ static int distill_launch(const void* z, int ztype, const DistillArgs& a, const 
     const int64_t pieces = (a.C + VEC - 1) / VEC;
     // As few pieces a thread as hold the row (one that no thread has costs what the others do: 4096x20000 bf16 73 us with 5 of 512 threads,
     // 106 with 8), and as few threads, so that several workgroups of a unit are at different steps.
-    if (pieces <= 64) return go(distill_row_kernel<T, 64, 1, MODE>, 64);
-    if (pieces <= 128) return go(distill_row_kernel<T, 64, 2, MODE>, 64);
-    if (pieces <= 256) return go(distill_row_kernel<T, 64, 4, MODE>, 64);
-    if (pieces <= 512) return go(distill_row_kernel<T, 256, 2, MODE>, 256);
-    if (pieces <= 1024) return go(distill_row_kernel<T, 256, 4, MODE>, 256);
-    if (pieces <= 1536) return go(distill_row_kernel<T, 256, 6, MODE>, 256);
-    if (pieces <= 2048) return go(distill_row_kernel<T, 256, 8, MODE>, 256);
-    if (pieces <= 2560) return go(distill_row_kernel<T, 256, 10, MODE>, 256);
-    if (pieces <= 3072) return go(distill_row_kernel<T, 512, 6, MODE>, 512);
-    if (pieces <= 3584) return go(distill_row_kernel<T, 512, 7, MODE>, 512);
-    if (pieces <= 4096) return go(distill_row_kernel<T, 512, 8, MODE>, 512);
-    if (pieces <= 6144) return go(distill_row_kernel<T, 1024, 6, MODE>, 1024);
+    if (pieces <= 64 * 1) return go(distill_row_kernel<T, 64, 1, MODE>, 64);
+    if (pieces <= 64 * 2) return go(distill_row_kernel<T, 64, 2, MODE>, 64);
+    if (pieces <= 64 * 4) return go(distill_row_kernel<T, 64, 4, MODE>, 64);
+    if (pieces <= 256 * 2) return go(distill_row_kernel<T, 256, 2, MODE>, 256);
+    if (pieces <= 256 * 4) return go(distill_row_kernel<T, 256, 4, MODE>, 256);
+    if (pieces <= 256 * 6) return go(distill_row_kernel<T, 256, 6, MODE>, 256);
+    if (pieces <= 256 * 8) return go(distill_row_kernel<T, 256, 8, MODE>, 256);
+    if (pieces <= 256 * 10) return go(distill_row_kernel<T, 256, 10, MODE>, 256);
+    if (pieces <= 512 * 6) return go(distill_row_kernel<T, 512, 6, MODE>, 512);
+    if (pieces <= 512 * 7) return go(distill_row_kernel<T, 512, 7, MODE>, 512);
+    if (pieces <= 512 * 8) return go(distill_row_kernel<T, 512, 8, MODE>, 512);
+    if (pieces <= 1024 * 6) return go(distill_row_kernel<T, 1024, 6, MODE>, 1024);
     return go(distill_row_kernel<T, 1024, 8, MODE>, 1024);
   });
 }

@@ -11,7 +11,6 @@
 // key is found by its bits instead, 8 at a time: topk_radix_row.
 // Few long rows are split into parts, one workgroup each, whose sorted lists a second launch merges.
 #include "rows.h"
-#include "quantize.h"
 #include "plan.h"
 
 typedef unsigned long long u64;
@@ -46,7 +45,7 @@ struct TopkShared {
   unsigned n, bin, need, wave[NT / 64];
 };
 
-// n candidates (all different) -> the places of the k largest; out(place, pair).  Begins and ends the reading of cand with a barrier.
+// n candidates (all different) -> the places of the k largest; out(place, pair).  The candidates are whole behind its barrier.
 template <int NT, class F>
 __device__ __forceinline__ void topk_place(u64* cand, int n, int k, F&& out) {
   typedef u64 u64x2 __attribute__((ext_vector_type(2)));
