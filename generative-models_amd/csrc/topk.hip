@@ -33,7 +33,7 @@ __device__ __forceinline__ unsigned topk_index(u64 pair) { return 0xFFFFFFFFu - 
 #define TOPK_SEGS 8      // segments of a thread: 16 take LDS from two of the 8 workgroups that a compute unit holds
 
 #define TOPK_WAVE 4096       // elements of a row that one wave takes at most
-#define TOPK_PART 4096       // elements of a part at least
+#define TOPK_PART 4096       // elements of a part that one round of loads of fp32 takes
 #define TOPK_PAIRS 4096      // pairs that a merge holds in LDS at most
 #define TOPK_BLOCKS 512      // workgroups that are worth having: a row has no more parts
 
@@ -273,26 +273,33 @@ __global__ __launch_bounds__(TOPK_NT) void topk_merge_kernel(const T* __restrict
     index[row * k + place] = (int)c;
   };
   // head at = h * parts + p: pair h of list p
-  constexpr int SLOTS = (4 * GMK_TOPK_MAX + TOPK_BLOCKS + 63) / 64;
+  // In registers, a loop over all of them for each bit: 4 slots of 64 heads where they hold them (5x150001, k = 50: 5.2 us of the merge, with all of them 9.4).
   const int heads = min(k, (4 * k + parts - 1) / parts), some = heads * parts;
-  unsigned m[SLOTS], bound = 0;
-  int p = lane % parts, h = lane / parts;   // 64 further on: 64 % parts lists and 64 / parts places
-  const int dp = 64 % parts, dh = 64 / parts;
+  unsigned bound = 0;
+  auto search = [&](auto slots) {
+    constexpr int SLOTS = decltype(slots)::value;
+    unsigned m[SLOTS];
+    int p = lane % parts, h = lane / parts;   // 64 further on: 64 % parts lists and 64 / parts places
+    const int dp = 64 % parts, dh = 64 / parts;
 #pragma unroll
-  for (int i = 0; i < SLOTS; ++i) {
-    m[i] = h < heads ? (unsigned)(pairs[p * k + h] >> 32) : 0u;
-    p += dp;
-    h += dh + (p >= parts ? 1 : 0);
-    p -= p >= parts ? parts : 0;
-  }
-  for (int bit = 31; bit >= 14; --bit) {
-    const unsigned up = bound | 1u << bit;
-    int have = 0;
+    for (int i = 0; i < SLOTS; ++i) {
+      m[i] = h < heads ? (unsigned)(pairs[p * k + h] >> 32) : 0u;
+      p += dp;
+      h += dh + (p >= parts ? 1 : 0);
+      p -= p >= parts ? parts : 0;
+    }
+    for (int bit = 31; bit >= 14; --bit) {
+      const unsigned up = bound | 1u << bit;
+      int have = 0;
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i)
-      if (i * 64 < some) have += __popcll(__ballot(m[i] >= up));
-    if (have >= k) bound = up;
-  }
+      for (int i = 0; i < SLOTS; ++i) have += __popcll(__ballot(m[i] >= up));
+      if (have >= k) bound = up;
+    }
+  };
+  constexpr int MOST = (4 * GMK_TOPK_MAX + TOPK_BLOCKS + 63) / 64;
+  if (some <= 4 * 64) search(std::integral_constant<int, 4>{});
+  else if (some <= 14 * 64) search(std::integral_constant<int, 14>{});
+  else search(std::integral_constant<int, MOST>{});
   for (int i = threadIdx.x; i < all; i += TOPK_NT)
     if ((unsigned)(pairs[i] >> 32) >= bound) {
       const unsigned at = atomicAdd(&s_n, 1u);
@@ -322,14 +329,16 @@ __global__ __launch_bounds__(TOPK_NT) void topk_merge_kernel(const T* __restrict
   }
 }
 
-// parts of a row: as many as give the card something to do, none shorter than TOPK_PART
+// parts of a row: as many as give the card something to do, none longer than a round of loads needs where that is few enough
 static int topk_parts(int64_t n, int64_t C, int k) {
   int64_t p = n < TOPK_BLOCKS ? TOPK_BLOCKS / n : 1;
-  const int64_t long_enough = C / TOPK_PART, fit = TOPK_PAIRS / k;
-  if (p > long_enough) p = long_enough;
+  const int64_t rounds = C < 2 * TOPK_PART ? 1 : (C + TOPK_PART - 1) / TOPK_PART, fit = TOPK_PAIRS / k;
+  if (p > rounds) p = rounds;
   if (p > fit) p = fit;
   return p < 2 ? 1 : (int)p;
 }
+// elements of all parts but the last, whole pieces of fp32; the last has at least C / parts - 4 parts > 2000 (and k <= 256)
+static int64_t topk_part_len(int64_t C, int parts) { return ((C + parts - 1) / parts + 3) / 4 * 4; }
 
 extern "C" size_t gmk_topk_rows_workspace_bytes(int64_t n, int64_t C, int k) {
   if (n <= 0 || C <= 0 || k <= 0 || k > GMK_TOPK_MAX) return 0;
@@ -349,7 +358,7 @@ extern "C" int gmk_topk_rows(const void* x, int xtype, void* value, int* index, 
               gmk_aligned_to(index, 4) && (parts == 1 || gmk_aligned16(ws)), GMK_E_ALIGN);
   GMK_REQUIRE(ws_bytes >= gmk_topk_rows_workspace_bytes(n, C, k), GMK_E_WORKSPACE);
   GMK_PLAN_HOOK(gmk_topk_rows, x, xtype, value, index, n, C, k, ws, ws_bytes, stream);
-  const int64_t len = parts == 1 ? C : (C + parts - 1) / parts / 8 * 8;   // of all parts but the last
+  const int64_t len = parts == 1 ? C : topk_part_len(C, parts);
   return gmk_with_dtype(xtype, [&](auto t) -> int {
     using T = decltype(t);
     const T* xt = (const T*)x;

@@ -39,6 +39,18 @@ def test_topk_rows(shape, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [8191, 8192, 8193, 12287, 12289, 24577, 2093057, 2097153])
+def test_topk_rows_where_parts_end(C, dtype):
+    """Rows around whole numbers of parts, the last one short; the largest elements in the last part, or in the first."""
+    for k in (1, 8, 50, 256):
+        x = _randn(C + k, 2, C)
+        x[0, C - min(k, 100):] += 20
+        x[1, : min(k, 100)] += 20
+        _check(x.to(dtype), k)
+
+
+@gpu
 @pytest.mark.parametrize("C,k", [(10, 4), (300, 40), (5000, 256), (70001, 64), (200000, 17)])
 def test_topk_rows_ties_and_masks(C, k):
     """Rows of equal values, of few different ones, masked to fewer than k, wholly masked, with NaN and both zeros, rising and
