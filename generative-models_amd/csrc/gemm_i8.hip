@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
   };
   // A wave's part of LDS for its epilogue; until then it holds the tile's scales and bias, which are loaded at the tile's start:
   // XS of its rows, LS each of its columns' scales and bias (zeros where there are none).
-  constexpr int LD = TN * 16, XS = TM * 16 < 64 ? 64 : TM * 16, LS = LD < 64 ? 64 : LD;
+  constexpr int LD = TN * 16, XS = (TM * 16 + 63) / 64 * 64, LS = LD < 64 ? 64 : LD;
   static_assert(XS + 2 * LS <= 16 * LD && XS % 64 == 0 && LS % 64 == 0, "the scales fit a wave's part");
   float* const part = (float*)(lds + S * BUF) + wave * 16 * LD;
   auto load_scales = [&](int m, int n) {
@@ -459,7 +459,8 @@ static int gemm_i8_check(int M, int K, int N, int ytype, int act) {
 //   64x32 tiles: up to 32 rows.  32x4096x32768 30.0 (64x64 31.2), but 64 rows 39.1 (31.9)
 //   beyond that, the least estimate of rounds * (start and end of a tile + 128-byte chunks of K * time of one), its constants
 //   measured with a unit full of that kernel: 64x64 512x4096x4096 16.3 (128x128 19.3), 128x128 with 8 waves 1024x4096x4096 22.0 (28.4, two
-//   workgroups of 4 waves 26.7), with 4 waves 2048x4096x4096 35.0 (40.3, 256x256 45.3), 256x256 4096x4096x4096 54 (64.5)
+//   workgroups of 4 waves 26.7), 128 columns by 192 rows 700x2048x7000 16.9 (19.4, 128x128 with 8 waves 22.7), 128x128 with 4 waves
+//   2048x4096x4096 35.0 (40.3, 256x256 45.3), 256x256 4096x4096x4096 54 (64.5)
 static int gemm_i8_launch(const signed char* xq, const float* xscale, const signed char* wq, const float* wscale,
                           const float* bias, void* y, int ytype, int M, int K, int N, int act, gmk_stream_t stream) {
   const int cus = i8_cus();
@@ -478,9 +479,11 @@ static int gemm_i8_launch(const signed char* xq, const float* xscale, const sign
     if (M <= 32) return go(gemm_i8_tile_launch<T, 64, 32, 2, 2, 6>);
     const float e64 = estimate(64, 64, 2, 4.f, 0.38f), e128 = estimate(128, 128, 1, 6.5f, 0.47f);
     const float e128x2 = estimate(128, 128, 2, 6.f, 0.9f), e256 = estimate(256, 256, 1, 10.f, 1.38f);
-    const float least = fminf(fminf(e64, e128), fminf(e128x2, e256));
+    const float e192 = estimate(128, 192, 1, 7.5f, 0.66f);
+    const float least = fminf(fminf(fminf(e64, e128), fminf(e128x2, e256)), e192);
     if (least == e64) return go(gemm_i8_tile_launch<T, 64, 64, 2, 2, 4>);
     if (least == e128) return go(gemm_i8_tile_launch<T, 128, 128, 4, 2, 4>);
+    if (least == e192) return go(gemm_i8_tile_launch<T, 128, 192, 4, 2, 3>);
     if (least == e128x2) return go(gemm_i8_tile_launch<T, 128, 128, 2, 2, 2>);
     return go(gemm_i8_tile_launch<T, 256, 256, 4, 2, 2>);
   });
