@@ -167,12 +167,13 @@ __device__ __forceinline__ float distill_most(const gmk_u32x4& v, float mx) {
   return mx;
 }
 
-// elements [e, C) of a row from a piece's values, as far as there are any
+// Elements [e, C) of a row from a piece's values, as far as there are any.  Whole pieces go past the caches, where the logits stay: 4096x32768
+// bf16 125 us (132), as two calls 193 (207); 1001x10007 fp32 19.0 (18.5), as two calls 30.1 (30.5).
 template <class T>
 __device__ __forceinline__ void distill_put(T* dzr, int64_t e, int64_t C, const float* o) {
   constexpr int VEC = gmk_elem<T>::VEC;
   if (e + VEC <= C) {
-    gmk_store16(dzr + e, gmk_pack<T>(o));
+    gmk_stream16(dzr + e, gmk_pack<T>(o));
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)

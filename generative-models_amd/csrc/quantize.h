@@ -2,7 +2,6 @@
 #pragma once
 #include "rows.h"
 
-
 // The largest magnitude of a row, as the bits of the type without their sign: their order as whole numbers is that of the magnitudes,
 // infinities and NaNs above all.  16-bit types two at a time.
 template <class T>
@@ -80,5 +79,5 @@ struct GmkQuant {
   }
 };
 
-int gmk_quantize_rows_launch(const void* x, int xtype, signed char* q, float* scale, int64_t M, int K, int ldq,
+int gmk_quantize_rows_launch(const void* x, int xtype, signed char* q, float* scale, int64_t M, int K, int ldq, bool once,
                              gmk_stream_t stream);

@@ -12,7 +12,7 @@
 
 // NT threads a row, ROWS rows a workgroup.  A thread keeps its first KEEP pieces in registers between the maximum and the rounding: rows up
 // to KEEP * NT pieces are read from memory once, longer ones read their rest again.
-template <class T, int NT, int ROWS, int KEEP>
+template <class T, int NT, int ROWS, int KEEP, bool STREAM = false>
 __global__ __launch_bounds__(NT * ROWS) void quantize_rows_kernel(const T* __restrict__ x, signed char* __restrict__ q,
                                                                   float* __restrict__ scale, int64_t M, int K, int ldq) {
   constexpr int VEC = gmk_elem<T>::VEC;
@@ -28,7 +28,7 @@ __global__ __launch_bounds__(NT * ROWS) void quantize_rows_kernel(const T* __res
   const int e0 = t * VEC;
 #pragma unroll
   for (int i = 0; i < KEEP; ++i)
-    if (e0 + i * NT * VEC < K) keep[i] = gmk_row_piece(xr, e0 + i * NT * VEC, K, 0.f);
+    if (e0 + i * NT * VEC < K) keep[i] = gmk_row_piece<STREAM>(xr, e0 + i * NT * VEC, K, 0.f);
 #pragma unroll
   for (int i = 0; i < KEEP; ++i)
     if (e0 + i * NT * VEC < K) mag.scan(keep[i]);
@@ -49,7 +49,8 @@ __global__ __launch_bounds__(NT * ROWS) void quantize_rows_kernel(const T* __res
 // 1024 threads a row where there are too few rows to fill the card and a row has work for them; a wave a row where rows are short
 // (8192x512 bf16: 6.2 us, with 256 threads 10.1); else 256 threads (8192x2048 fp32: 17.4 us, a wave a row 28.0).  Bound by memory with many
 // rows (8192x4096 bf16: 20.9 us, 4.8 TB/s in and out), by latency with few (256x4096 fp32: 3.8 us, an empty launch 2.6).
-int gmk_quantize_rows_launch(const void* x, int xtype, signed char* q, float* scale, int64_t M, int K, int ldq,
+// `once`: x is read past the caches, for the sake of what the caller needs in them afterwards (8192x4096 bf16 alone 24.0 us).
+int gmk_quantize_rows_launch(const void* x, int xtype, signed char* q, float* scale, int64_t M, int K, int ldq, bool once,
                              gmk_stream_t stream) {
   return gmk_with_dtype(xtype, [&](auto t) -> int {
     using T = decltype(t);
@@ -62,6 +63,7 @@ int gmk_quantize_rows_launch(const void* x, int xtype, signed char* q, float* sc
     };
     if (M <= 512 && K > 256 * VEC) return go(quantize_rows_kernel<T, 1024, 1, 4>, M, 1024);
     if (K <= 128 * VEC) return go(quantize_rows_kernel<T, 64, 4, 2>, (M + 3) / 4, 256);
+    if (once) return go(quantize_rows_kernel<T, 256, 1, 4, true>, M, 256);
     return go(quantize_rows_kernel<T, 256, 1, 4>, M, 256);
   });
 }
@@ -75,5 +77,5 @@ extern "C" int gmk_quantize_rows(const void* x, int xtype, signed char* q, float
   GMK_REQUIRE(x && q && scale, GMK_E_NULL);
   GMK_REQUIRE(gmk_aligned_to(x, gmk_dtype_size(xtype)) && gmk_aligned16(q) && gmk_aligned_to(scale, 4), GMK_E_ALIGN);
   GMK_PLAN_HOOK(gmk_quantize_rows, x, xtype, q, scale, M, K, ldq, stream);
-  return gmk_quantize_rows_launch(x, xtype, q, scale, M, K, ldq, stream);
+  return gmk_quantize_rows_launch(x, xtype, q, scale, M, K, ldq, false, stream);
 }

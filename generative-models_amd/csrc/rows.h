@@ -26,15 +26,18 @@ static inline auto gmk_with_dtype(int t, F&& f) {
 }
 
 // A 16-byte piece of a row, from any address that is aligned to the element: rows of odd lengths start anywhere, and gfx950
-// reads and writes 16 bytes at any alignment.
-template <class T>
+// reads and writes 16 bytes at any alignment.  STREAM: the piece is not worth a place in the caches.
+typedef unsigned gmk_u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+template <bool STREAM = false, class T>
 __device__ __forceinline__ gmk_u32x4 gmk_load16(const T* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load((const gmk_u32x4_at2*)p);
   gmk_u32x4 v;
   __builtin_memcpy(&v, p, 16);
   return v;
 }
+// past the caches
 template <class T>
-__device__ __forceinline__ void gmk_store16(T* p, const gmk_u32x4& v) { __builtin_memcpy(p, &v, 16); }
+__device__ __forceinline__ void gmk_stream16(T* p, const gmk_u32x4& v) { __builtin_nontemporal_store((gmk_u32x4_at2)v, (gmk_u32x4_at2*)p); }
 
 // element i (a constant) of a piece, as fp32
 template <class T>
@@ -68,10 +71,10 @@ __device__ __forceinline__ gmk_u32x4 gmk_pack(const float* f) {
 
 // The piece of a row that starts at element e: whole pieces in one load, the last, partial one element by element, its
 // missing elements `fill` (-inf leaves a maximum and a sum of exponentials as they are, 0 a largest magnitude).
-template <class T>
+template <bool STREAM = false, class T>
 __device__ __forceinline__ gmk_u32x4 gmk_row_piece(const T* row, int64_t e, int64_t C, float fill = -__builtin_inff()) {
   constexpr int VEC = gmk_elem<T>::VEC;
-  if (e + VEC <= C) return gmk_load16(row + e);
+  if (e + VEC <= C) return gmk_load16<STREAM>(row + e);
   T t[VEC];
   if (e >= C) {
 #pragma unroll

@@ -162,6 +162,17 @@ def test_gemm_i8_larger_kernels(shape):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,M,K,N", [(torch.bfloat16, 9001, 4100, 130), (torch.float32, 4500, 4097, 300), (torch.float16, 700, 8200, 12000)])
+def test_linear_i8_large_is_its_two_steps(dtype, M, K, N):
+    """Sizes at which the activations pass the caches by: the same bits as quantize_rows and matmul_i8."""
+    from gmk import ops
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.randn(M, K, generator=g, device="cuda").to(dtype)
+    wq, ws = ops.quantize_rows(torch.randn(N, K, generator=g, device="cuda"))
+    assert torch.equal(ops.linear_i8(x, wq, ws, act="relu"), ops.matmul_i8(*ops.quantize_rows(x), wq, ws, act="relu", out_dtype=dtype))
+
+
+@gpu
 @pytest.mark.parametrize("M", [1, 4, 20, 150])
 def test_linear_i8_rows_are_independent_and_nan_stays_in_its_row(M):
     from gmk import ops
