@@ -11,6 +11,11 @@
 // many long ones for the loss alone, are taken in parts: the parts' maxima and sums (distill_part_kernel), then everything else, each part's workgroup joining them
 // again (distill_grad_kernel, which is the backward pass too).  The gradient of the listed classes is written over what the dense pass
 // wrote, by the workgroup that wrote it.
+//
+// Measured: 4096x32768 bf16 with labels 125 us, 4.3 TB/s in and out; without them, one exponential less for each logit and for each
+// gradient, 104.5 us and 5.1 TB/s (a copy 5.1 to 5.5): bound by the vector units, then by memory.  1001x10007 fp32 19 us, as loss and
+// backward pass 12 + 18.  256x10 5.1 us, a launch and the
+// latency of its chain of loads and reductions; 9x200003 fp16 10.9 us, two launches.
 #include "rows.h"
 #include "plan.h"
 

@@ -49,6 +49,11 @@ __device__ __forceinline__ void i8_stream4(const float4& z, T* p) {
 // one piece of as many consecutive rows together touch every bank once.  LDS is filled in lane order, so it is the address in memory
 // that is permuted: a row's lanes still read its BK bytes in one go.
 // Rows behind the last one and pieces behind K are past the buffer's end for the load, which makes them zeros.
+//
+// Measured, bf16 out: 8192x8192x8192 409 to 420 us, 2620 to 2690 TOP/s (a copy-free loop of the instruction reaches 4000 to 4350);
+// 8192x4096x16384 446 us with the quantiser, 427 for the product.  The matrix cores are busy in 59 % (K = 4096) to 69 % (K = 8192) of the
+// cycles, at the 1.9 GHz that the card holds under this load; LDS has no bank conflict.  What is left is the end of a tile, when all
+// units write their 128 KB at once: 8192x1024x16384 takes 155 us of which the products are 90.
 #define I8_BK 128
 __device__ __forceinline__ int i8_place(int row, int piece) { return piece ^ (row & 7); }
 
@@ -322,6 +327,7 @@ static int gemm_i8_tile_launch(const signed char* xq, const float* xscale, const
 // A workgroup makes NT * 16 columns times 16 rows of y; its waves take turns along K, 64 bytes of each row at a time straight from
 // memory into the instruction's registers, U steps in flight, and their sums meet in LDS.  Rows behind the last one are read from the
 // last one and never stored; behind K the weight's piece is zero.
+// Bound by the weight's bytes: 1x4096x32768 bf16 30.1 us, 4.5 TB/s with the start of the launch, 28.1 from 8-bit rows.
 // X is the rows' type: 8-bit values with xscale, or, for at most I8_FUSED_ROWS rows of floating numbers, x itself, which every workgroup
 // then quantises into its LDS while its first weights are on their way: one launch instead of two.
 #define I8_FUSED_ROWS 4
