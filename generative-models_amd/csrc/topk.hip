@@ -11,9 +11,9 @@
 // key is found by its bits instead, 8 at a time: topk_radix_row.
 // Few long rows are split into parts, one workgroup each, whose sorted lists a second launch merges.
 //
-// Measured: 2048x65536 bf16, k = 32 67.3 us, 4.0 TB/s of the row's bytes (a maximum over them reads 4.8; a tenth of the bytes is read
-// twice); 256x1000 fp32, k = 10 5.3 us and 5x150001 fp32, k = 50 11.7 us, both the latency of one and of two launches' chains of loads, search and
-// counting.
+// Measured: 2048x65536 bf16, k = 32 54.4 us, 4.9 TB/s of the rows' bytes, which is what a maximum over them reads at; 256x1000 fp32, k = 10
+// 4.7 us and 5x150001 fp32, k = 50 11.6 us, the latency of one and of two launches' chains of loads, search and counting.  With few threads a
+// row (512x200000 fp16, k = 128: 59.6 us, 3.4 TB/s) by the loads that are in flight.
 #include "rows.h"
 #include "plan.h"
 
@@ -136,30 +136,26 @@ __device__ __forceinline__ void topk_row(const T* __restrict__ x, int64_t C, uns
   static_assert(MX * NT * 4 <= (int)sizeof(sh.cand), "the maxima fit");
   constexpr int64_t LOAD = (int64_t)NT * VEC, GROUP = LOAD * TOPK_LOADS;   // elements of one load of all threads; of one round of loads
   const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t groups = (C + GROUP - 1) / GROUP, per_seg = (groups + TOPK_SEGS - 1) / TOPK_SEGS;   // rounds; of a segment
+  const int64_t groups = (C + GROUP - 1) / GROUP, per_seg = (groups + TOPK_SEGS - 1) / TOPK_SEGS;   // rounds; of a segment: one load where
+  static_assert(TOPK_SEGS == 2 * TOPK_LOADS, "segments of up to two rounds");                      // there are at most two rounds
+  const unsigned pieces = groups <= 2 ? 1u : (unsigned)per_seg * TOPK_LOADS;                        // of a segment
   const float low = -__builtin_inff();
   float best[MX];
 #pragma unroll
   for (int i = 0; i < MX; ++i) best[i] = low;
   const int64_t e0 = (int64_t)tid * VEC;
   gmk_u32x4 v[TOPK_LOADS];   // behind the loop: the last round, which is all of a short row
-  for (int64_t g = 0, s = 0; g < groups; g += per_seg, ++s) {
-    float mine[MX];
+  auto load = [&](int64_t h) {
+    const int64_t e = e0 + h * GROUP;
+    if ((h + 1) * GROUP <= C) {
 #pragma unroll
-    for (int i = 0; i < MX; ++i) mine[i] = low;
-    const int64_t end = g + per_seg < groups ? g + per_seg : groups;
-    for (int64_t h = g; h < end; ++h) {
-      const int64_t e = e0 + h * GROUP;
-      if ((h + 1) * GROUP <= C) {
+      for (int i = 0; i < TOPK_LOADS; ++i) v[i] = gmk_load16(x + e + i * LOAD);
+    } else {
 #pragma unroll
-        for (int i = 0; i < TOPK_LOADS; ++i) v[i] = gmk_load16(x + e + i * LOAD);
-      } else {
-#pragma unroll
-        for (int i = 0; i < TOPK_LOADS; ++i) v[i] = gmk_row_piece(x, e + i * LOAD, C);
-      }
-#pragma unroll
-      for (int i = 0; i < TOPK_LOADS; ++i) topk_most<T, MX>(v[i], mine);
+      for (int i = 0; i < TOPK_LOADS; ++i) v[i] = gmk_row_piece(x, e + i * LOAD, C);
     }
+  };
+  auto close = [&](const float* mine, int64_t s) {   // segment s of this thread
     float all = mine[0];
 #pragma unroll
     for (int i = 0; i < MX; ++i) {
@@ -167,6 +163,33 @@ __device__ __forceinline__ void topk_row(const T* __restrict__ x, int64_t C, uns
       all = __builtin_elementwise_maximum(all, mine[i]);
     }
     sh.seg[s][tid] = all;
+  };
+  float mine[MX];
+  auto open = [&]() {
+#pragma unroll
+    for (int i = 0; i < MX; ++i) mine[i] = low;
+  };
+  if (groups <= 2) {
+    for (int64_t h = 0; h < groups; ++h) {
+      load(h);
+#pragma unroll
+      for (int i = 0; i < TOPK_LOADS; ++i) {
+        open();
+        topk_most<T, MX>(v[i], mine);
+        close(mine, h * TOPK_LOADS + i);
+      }
+    }
+  } else {
+    for (int64_t g = 0, s = 0; g < groups; g += per_seg, ++s) {
+      open();
+      const int64_t end = g + per_seg < groups ? g + per_seg : groups;
+      for (int64_t h = g; h < end; ++h) {
+        load(h);
+#pragma unroll
+        for (int i = 0; i < TOPK_LOADS; ++i) topk_most<T, MX>(v[i], mine);
+      }
+      close(mine, s);
+    }
   }
   unsigned* const maxima = (unsigned*)sh.cand;
 #pragma unroll
@@ -192,7 +215,7 @@ __device__ __forceinline__ void topk_row(const T* __restrict__ x, int64_t C, uns
   unsigned again = 0;   // segments of this thread that reach it
   if (groups > 1)
     for (int i = 0; i < TOPK_SEGS; ++i)
-      if (i * per_seg < groups && !(sh.seg[i][tid] < limit)) again |= 1u << i;
+      if ((groups == 2 || i * per_seg < groups) && !(sh.seg[i][tid] < limit)) again |= 1u << i;
   __syncthreads();
   auto collect = [&](const gmk_u32x4& v, int64_t e) {
 #pragma unroll
@@ -220,7 +243,7 @@ __device__ __forceinline__ void topk_row(const T* __restrict__ x, int64_t C, uns
     if (hits > TOPK_CAND(NT)) {
       if (tid == 0) sh.n = hits;
     } else {
-      const unsigned pieces = (unsigned)per_seg * TOPK_LOADS, all = hits * pieces;   // < 2^31 elements of a row
+      const unsigned all = hits * pieces;   // < 2^29
       for (unsigned q = tid; q < all; q += NT * TOPK_LOADS) {
         gmk_u32x4 v[TOPK_LOADS];
         int64_t e[TOPK_LOADS];
@@ -385,8 +408,9 @@ extern "C" int gmk_topk_rows(const void* x, int xtype, void* value, int* index, 
     using T = decltype(t);
     const T* xt = (const T*)x;
     hipStream_t st = (hipStream_t)stream;
-    // One maximum a thread where that makes at least twice k of them, else four.  A wave a row for short rows: 8192x1000 fp32 15.5 us, 256
-    // threads 28; 4096x4096 bf16, k = 64 21.5 (26), but 256 rows of that 13.5 (7.9).
+    // One maximum a thread where that makes at least twice k of them, else four.  A wave a row for rows of a few pieces a thread, of more
+    // where the card is full of rows: 8192x1000 fp32 13.0 us, 256 threads 22.7; 4096x4096 bf16, k = 64 16.6 (24.3), but 1024x4000 fp32 12.9
+    // (9.7) and 256x1000 fp32 5.2 (4.7).
     const bool many = k <= TOPK_NT / 2 && len >= (int64_t)2 * k * gmk_elem<T>::VEC;
     if (parts == 1) {
       auto go = [&](auto kernel, int nt) -> int {
@@ -395,7 +419,7 @@ extern "C" int gmk_topk_rows(const void* x, int xtype, void* value, int* index, 
         GMK_CHECK_LAUNCH();
         return GMK_OK;
       };
-      if (k <= 64 && (C <= 1024 || (C <= TOPK_WAVE && n >= 1024))) return go(topk_rows_kernel<T, 64, 4>, 64);
+      if (k <= 64 && C <= (n >= 2048 ? TOPK_WAVE : TOPK_WAVE / 8)) return go(topk_rows_kernel<T, 64, 4>, 64);
       if (many) return go(topk_rows_kernel<T, TOPK_NT, 1>, TOPK_NT);
       return go(topk_rows_kernel<T, TOPK_NT, 4>, TOPK_NT);
     }
