@@ -12,8 +12,8 @@
 // Few long rows are split into parts, one workgroup each, whose sorted lists a second launch merges.
 //
 // Measured: 2048x65536 bf16, k = 32 54.4 us, 4.9 TB/s of the rows' bytes, which is what a maximum over them reads at; 256x1000 fp32, k = 10
-// 4.7 us and 5x150001 fp32, k = 50 11.6 us, the latency of one and of two launches' chains of loads, search and counting.  With few threads a
-// row (512x200000 fp16, k = 128: 59.6 us, 3.4 TB/s) by the loads that are in flight.
+// 4.7 us and 5x150001 fp32, k = 50 11.6 us, the latency of one and of two launches' chains of loads, search and counting.  What
+// is read again grows with k: 512x200000 fp16 40.4 us with k = 10 (5.1 TB/s), 59.6 with k = 128.
 #include "rows.h"
 #include "plan.h"
 
@@ -39,7 +39,7 @@ __device__ __forceinline__ unsigned topk_index(u64 pair) { return 0xFFFFFFFFu - 
 #define TOPK_WAVE 4096       // elements of a row that one wave takes at most
 #define TOPK_PART 4096       // elements of a part that one round of loads of fp32 takes
 #define TOPK_PAIRS 4096      // pairs that a merge holds in LDS at most
-#define TOPK_BLOCKS 512      // workgroups that are worth having: a row has no more parts
+#define TOPK_BLOCKS 512      // workgroups that are worth having, a row has no more parts: 300x60000 fp32, k = 50 17.7 us (with 1024 22.1)
 
 template <int NT>
 struct TopkShared {

@@ -578,6 +578,14 @@ def _stream_of(dev):
     return _cur_stream if _cur_stream is not None else torch._C._cuda_getCurrentRawStream(dev)
 
 
+def _new_rows(n, C, device, dtype):
+    """An output (n, C), or (n,) with C = 0.  (empty_strided: empty costs half a microsecond more, and the smallest calls are all host time.)"""
+    t = torch.empty_strided((n, C) if C else (n,), (C, 1) if C else (1,), device=device, dtype=dtype)
+    if _rec_keep is not None:
+        _rec_keep.append(t)
+    return t
+
+
 @functools.lru_cache(maxsize=1024)
 def _scratch_bytes(name, *sizes):
     return int(getattr(lib(), name)(*sizes))
@@ -586,7 +594,7 @@ def _scratch_bytes(name, *sizes):
 def _scratch(device, name, *sizes):
     """(tensor or None, its bytes) of the scratch that an entry point asks for."""
     nbytes = _scratch_bytes(name, *sizes)
-    return (_new(nbytes, device, torch.uint8), nbytes) if nbytes else (None, 0)
+    return (_new_rows(nbytes, 0, device, torch.uint8), nbytes) if nbytes else (None, 0)
 
 
 def quantize_rows(x):
@@ -597,8 +605,8 @@ def quantize_rows(x):
     if K == 0:
         raise ValueError("x must have at least one column")
     ld = -(-K // 16) * 16
-    q = _new((M, ld), x.device, torch.int8)
-    scale = _new((M,), x.device, torch.float32)
+    q = _new_rows(M, ld, x.device, torch.int8)
+    scale = _new_rows(M, 0, x.device, torch.float32)
     check(lib().gmk_quantize_rows(_p(x), _FLOAT_IDS[x.dtype], _p(q), _p(scale), M, K, ld, _stream_of(dev)))
     return q, scale
 
@@ -626,7 +634,7 @@ def matmul_i8(xq, xscale, wq, wscale, bias=None, act=None, out_dtype=torch.float
         raise ValueError(f"xq has {K} columns: rows of 8-bit values are padded to a multiple of 16 (quantize_rows)")
     _chk_rows("xscale", xscale, _FP32, (M,), dev)
     N = _i8_args(dev, K, wq, wscale, bias, out_dtype)
-    y = _new((M, N), xq.device, out_dtype)
+    y = _new_rows(M, N, xq.device, out_dtype)
     check(lib().gmk_gemm_i8(_p(xq), _p(xscale), _p(wq), _p(wscale), _p(bias), _p(y), _FLOAT_IDS[out_dtype], M, K, N, act_id(act),
                             _stream_of(dev)))
     return y
@@ -639,7 +647,7 @@ def linear_i8(x, wq, wscale, bias=None, act=None, out_dtype=None):
     out_dtype = x.dtype if out_dtype is None else out_dtype
     M, K = x.shape
     N = _i8_args(dev, K, wq, wscale, bias, out_dtype)
-    y = _new((M, N), x.device, out_dtype)
+    y = _new_rows(M, N, x.device, out_dtype)
     ws, nbytes = _scratch(x.device, "gmk_linear_i8_workspace_bytes", M, K, N)
     check(lib().gmk_linear_i8_fwd(_p(x), _FLOAT_IDS[x.dtype], _p(wq), _p(wscale), _p(bias), _p(y), _FLOAT_IDS[out_dtype], M, K, N,
                                   act_id(act), _p(ws), nbytes, _stream_of(dev)))
@@ -654,8 +662,8 @@ def topk_rows(x, k):
     k = int(k)
     if not 1 <= k <= min(C, TOPK_MAX):
         raise ValueError(f"k must be between 1 and min({C} columns, {TOPK_MAX}), not {k}")
-    value = _new((n, k), x.device, x.dtype)
-    index = _new((n, k), x.device, torch.int32)
+    value = _new_rows(n, k, x.device, x.dtype)
+    index = _new_rows(n, k, x.device, torch.int32)
     ws, nbytes = _scratch(x.device, "gmk_topk_rows_workspace_bytes", n, C, k)
     check(lib().gmk_topk_rows(_p(x), _FLOAT_IDS[x.dtype], _p(value), _p(index), n, C, k, _p(ws), nbytes, _stream_of(dev)))
     return value, index
@@ -687,8 +695,8 @@ def distill_fwd(logits, teacher, index, labels=None, T=1.0, soft=1.0, hard=0.0):
     soft T^2 KL(softmax(teacher / T) || softmax(logits / T)) + hard CE(logits, labels).  Returns (loss (n,), stats (n, 3)), stats
     for distill_bwd."""
     n, C, k, dev = _distill_args(logits, teacher, index, labels, T, soft, hard)
-    loss = _new((n,), logits.device, torch.float32)
-    stats = _new((n, 3), logits.device, torch.float32)
+    loss = _new_rows(n, 0, logits.device, torch.float32)
+    stats = _new_rows(n, 3, logits.device, torch.float32)
     ws, nbytes = _scratch(logits.device, "gmk_distill_workspace_bytes", n, C)
     check(lib().gmk_distill_fwd(_p(logits), _FLOAT_IDS[logits.dtype], _p(teacher), _FLOAT_IDS[teacher.dtype], _p(index), _p(labels),
                                 _p(loss), _p(stats), n, C, k, float(T), float(soft), float(hard), _p(ws),
@@ -713,7 +721,7 @@ def distill_fwd_bwd(logits, teacher, index, labels=None, T=1.0, soft=1.0, hard=0
     n, C, k, dev = _distill_args(logits, teacher, index, labels, T, soft, hard)
     if weight is not None:
         _chk_rows("weight", weight, _FP32, (n,), dev)
-    loss = _new((n,), logits.device, torch.float32)
+    loss = _new_rows(n, 0, logits.device, torch.float32)
     dz = _new_like(logits)
     ws, nbytes = _scratch(logits.device, "gmk_distill_workspace_bytes", n, C)
     check(lib().gmk_distill_fwd_bwd(_p(logits), _FLOAT_IDS[logits.dtype], _p(teacher), _FLOAT_IDS[teacher.dtype], _p(index),
