@@ -172,13 +172,16 @@ __device__ __forceinline__ float distill_most(const gmk_u32x4& v, float mx) {
   return mx;
 }
 
-// Elements [e, C) of a row from a piece's values, as far as there are any.  Whole pieces go past the caches, where the logits stay: 4096x32768
-// bf16 125 us (132), as two calls 193 (207); 1001x10007 fp32 19.0 (18.5), as two calls 30.1 (30.5).
+// Elements [e, C) of a row from a piece's values, as far as there are any.  `stream`: whole pieces go past the caches, where the logits stay.
+// For the backward pass always (with the loss before it 4096x32768 bf16 193 us, else 207; 8000x8001 fp16 91.6, else 99.8); in one call with
+// the loss, which has no more use for the logits, where rows are whole lines of 128 bytes (4096x32768 bf16 125, else 132; 8000x8001 fp16
+// would take 67, else 61.5).
 template <class T>
-__device__ __forceinline__ void distill_put(T* dzr, int64_t e, int64_t C, const float* o) {
+__device__ __forceinline__ void distill_put(T* dzr, int64_t e, int64_t C, const float* o, bool stream) {
   constexpr int VEC = gmk_elem<T>::VEC;
   if (e + VEC <= C) {
-    gmk_stream16(dzr + e, gmk_pack<T>(o));
+    if (stream) gmk_store16<true>(dzr + e, gmk_pack<T>(o));
+    else gmk_store16<false>(dzr + e, gmk_pack<T>(o));
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
@@ -198,11 +201,12 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(const T* __restrict__ z
   const T* zr = z + row * a.C;
   T* dzr = dz + row * a.C;
   const int64_t e0 = (int64_t)threadIdx.x * VEC;
+  const bool lines = (((uintptr_t)dz | (uintptr_t)(a.C * (int64_t)sizeof(T))) & 127) == 0;
   const float w = MODE == 2 && weight ? weight[row] : 1.f;
   if (MODE == 2 && w == 0.f) {
     float o[VEC] = {};
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) distill_put(dzr, e0 + (int64_t)i * NT * VEC, a.C, o);
+    for (int i = 0; i < KEEP; ++i) distill_put(dzr, e0 + (int64_t)i * NT * VEC, a.C, o, lines);
     if (threadIdx.x == 0) loss[row] = 0.f;
     return;
   }
@@ -245,7 +249,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(const T* __restrict__ z
     for (int i = 0; i < KEEP; ++i) {
       float o[VEC];
       g.piece<T>(a, keep[i], o);
-      distill_put(dzr, e0 + (int64_t)i * NT * VEC, a.C, o);
+      distill_put(dzr, e0 + (int64_t)i * NT * VEC, a.C, o, lines);
     }
     __syncthreads();
     if (threadIdx.x < 64) distill_listed(a, en, g, dzr, 0, a.C);
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(const T* __restrict__ 
   if (MODE != 0 && w == 0.f) {
     float o[VEC] = {};
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) distill_put(dzr, e0 + i * NT * VEC, a.C, o);
+    for (int i = 0; i < KEEP; ++i) distill_put(dzr, e0 + i * NT * VEC, a.C, o, true);
     if (MODE == 2 && from == 0 && threadIdx.x == 0) loss[row] = 0.f;
     return;
   }
@@ -371,7 +375,7 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(const T* __restrict__ 
     for (int i = 0; i < KEEP; ++i) {
       float o[VEC];
       g.piece<T>(a, keep[i], o);
-      distill_put(dzr, e0 + i * NT * VEC, a.C, o);
+      distill_put(dzr, e0 + i * NT * VEC, a.C, o, true);
     }
     __syncthreads();
     if (threadIdx.x < 64) distill_listed(a, en, g, dzr, from, from + (int64_t)NT * KEEP * VEC);

@@ -31,13 +31,15 @@ __device__ __forceinline__ void i8_put4(const float4& z, T* p, int have) {   // 
   }
 }
 
-// All 4, past the caches, where the operands' tiles stay instead: 8192x4096x16384 454 us (470), 2048x4096x4096 35.7 (37.4), and two layers
-// one after the other 86.1 (87.9).
+// All 4, past the caches, where the operands' tiles stay instead: 8192x4096x16384 446 us (455), 1053x432x29312 33.5 (36.4).  Only where
+// rows are whole lines of 128 bytes: parts of a line that the caches do not join cost 2204x256x29857 81.8 us (43.0).
 template <class T>
 __device__ __forceinline__ void i8_stream4(const float4& z, T* p) {
   typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
   T4 t = {(T)z.x, (T)z.y, (T)z.z, (T)z.w};
+  asm volatile("");   // or the compiler makes one store of this and another branch's, without the hint
   __builtin_nontemporal_store(t, (T4*)p);
+  asm volatile("");
 }
 
 // ---- tiles through LDS -------------------------------------------------------------------------------------------------------
@@ -51,7 +53,7 @@ __device__ __forceinline__ void i8_stream4(const float4& z, T* p) {
 // Rows behind the last one and pieces behind K are past the buffer's end for the load, which makes them zeros.
 //
 // Measured, bf16 out: 8192x8192x8192 409 to 420 us, 2620 to 2690 TOP/s (a copy-free loop of the instruction reaches 4000 to 4350);
-// 8192x4096x16384 446 us with the quantiser, 427 for the product.  The matrix cores are busy in 59 % (K = 4096) to 69 % (K = 8192) of the
+// 8192x4096x16384 446 us, with the quantiser before it too (what that leaves in the caches).  The matrix cores are busy in 59 % (K = 4096) to 69 % (K = 8192) of the
 // cycles, at the 1.9 GHz that the card holds under this load; LDS has no bank conflict.  What is left is the end of a tile, when all
 // units write their 128 KB at once: 8192x1024x16384 takes 155 us of which the products are 90.
 #define I8_BK 128
@@ -248,6 +250,7 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
     const int n = n0 + wn + col;
     const bool common = act == GMK_ACT_NONE || act == GMK_ACT_RELU || act == GMK_ACT_GELU;
     const bool whole = m0 + wm + TM * 16 <= M && n0 + wn + LD <= N;
+    const bool lines = (((uintptr_t)y | (uintptr_t)((int64_t)N * sizeof(T))) & 127) == 0;
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
 #pragma unroll
@@ -273,11 +276,17 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
 #pragma unroll
           for (int u = 0; u < 16 / STEP; ++u) z[u] = make_float4(z[u].x > 0.f ? z[u].x : 0.f, z[u].y > 0.f ? z[u].y : 0.f, z[u].z > 0.f ? z[u].z : 0.f, z[u].w > 0.f ? z[u].w : 0.f);
         }
+        T* const yq = y + (int64_t)(mb + q0) * N + n;
+        if (whole && lines) {
 #pragma unroll
-        for (int u = 0; u < 16 / STEP; ++u) {
-          const int m = mb + q0 + u * STEP;
-          if (whole) i8_stream4<T>(z[u], y + (int64_t)m * N + n);
-          else if (m < M && n < N) i8_put4<T>(z[u], y + (int64_t)m * N + n, N - n);
+          for (int u = 0; u < 16 / STEP; ++u) i8_stream4<T>(z[u], yq + (int64_t)u * STEP * N);
+        } else if (whole) {
+#pragma unroll
+          for (int u = 0; u < 16 / STEP; ++u) i8_put4<T>(z[u], yq + (int64_t)u * STEP * N, 4);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 16 / STEP; ++u)
+            if (mb + q0 + u * STEP < M && n < N) i8_put4<T>(z[u], yq + (int64_t)u * STEP * N, N - n);
         }
       } else {   // a rarer activation: one value a lane
 #pragma unroll 1

@@ -35,9 +35,16 @@ __device__ __forceinline__ gmk_u32x4 gmk_load16(const T* p) {
   __builtin_memcpy(&v, p, 16);
   return v;
 }
-// past the caches
-template <class T>
-__device__ __forceinline__ void gmk_stream16(T* p, const gmk_u32x4& v) { __builtin_nontemporal_store((gmk_u32x4_at2)v, (gmk_u32x4_at2*)p); }
+template <bool STREAM, class T>
+__device__ __forceinline__ void gmk_store16(T* p, const gmk_u32x4& v) {
+  if constexpr (STREAM) {
+    asm volatile("");   // or the compiler makes one store of this and another branch's, without the hint
+    __builtin_nontemporal_store((gmk_u32x4_at2)v, (gmk_u32x4_at2*)p);
+    asm volatile("");
+  } else {
+    __builtin_memcpy(p, &v, 16);
+  }
+}
 
 // element i (a constant) of a piece, as fp32
 template <class T>
