@@ -53,9 +53,9 @@ __device__ __forceinline__ void i8_stream4(const float4& z, T* p) {
 // Rows behind the last one and pieces behind K are past the buffer's end for the load, which makes them zeros.
 //
 // Measured, bf16 out: 8192x8192x8192 409 to 420 us, 2620 to 2690 TOP/s (a copy-free loop of the instruction reaches 4000 to 4350);
-// 8192x4096x16384 446 us, with the quantiser before it too (what that leaves in the caches).  The matrix cores are busy in 59 % (K = 4096) to 69 % (K = 8192) of the
-// cycles, at the 1.9 GHz that the card holds under this load; LDS has no bank conflict.  What is left is the end of a tile, when all
-// units write their 128 KB at once: 8192x1024x16384 takes 155 us of which the products are 90.
+// 8192x4096x16384 446 us, with the quantiser before it too (its q is still in the caches).  The matrix cores are busy in 59 % (K = 4096) to
+// 69 % (K = 8192) of the cycles, at the 1.9 GHz that the card holds under this load; LDS has no bank conflict.  What is left is the end of a
+// tile, when all units write their 128 KB at once: 8192x1024x16384 takes 155 us of which the products are 90.
 #define I8_BK 128
 __device__ __forceinline__ int i8_place(int row, int piece) { return piece ^ (row & 7); }
 

@@ -133,7 +133,8 @@ def distillation_loss(outputs, value, index, labels=None, T=4.0, soft=0.9, hard=
     """Loss of each sample (n,) of a student's logits (n, C): soft T^2 KL(teacher || student) at temperature T over the teacher's kept logits
     `value` (n, k) of the classes `index` (n, k) int32 (gmk.ops.topk_rows; -1: no entry), plus hard * cross entropy where labels (n,) are
     given (outside [0, C): none).  CUDA tensors; outputs fp32, bf16 or fp16, under autograd.  In 32 bits the soft part is known to about
-    soft T^2 2^-20, so that it loses its digits at temperatures far above the logits' differences; the gradient keeps them."""
+    soft T^2 2^-20, so that it loses its digits at temperatures far above the logits' differences; the gradient keeps them.  As with any loss, a
+    backward pass is captured into a graph only while no eager graph of the same leaves is alive (torch.autograd's own rule)."""
     if labels is None:
         hard = 0.0
     return _DistillFn.apply(outputs.contiguous(), value.detach(), index, labels, float(T), float(soft), float(hard))

@@ -23,7 +23,7 @@ def _check(x, k, got=None):
     assert torch.equal(i.cpu().long(), ri), (x.shape, k)
     # the values are the row's own, bit for bit
     bits = torch.int32 if x.dtype == torch.float32 else torch.int16
-    assert torch.equal(v.cpu().view(bits), x.gather(1, ri).view(bits))
+    assert torch.equal(v.cpu().view(bits), x.view(bits).gather(1, ri))   # of whole numbers: a gather on the CPU changes a bf16 NaN's bits
 
 
 SHAPES = [(1, 1, 1), (3, 10, 3), (5, 10, 10), (256, 10, 3), (4, 63, 7), (2, 64, 64), (3, 65, 2), (7, 257, 256), (256, 1000, 10), (3, 1023, 100), (2, 2048, 128), (9, 4099, 33),
@@ -48,6 +48,37 @@ def test_topk_rows_where_parts_end(C, dtype):
         x[0, C - min(k, 100):] += 20
         x[1, : min(k, 100)] += 20
         _check(x.to(dtype), k)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C,k", [(9001, 100), (17001, 20), (33003, 40), (70001, 128)])
+def test_topk_rows_ties_and_masks_in_whole_rows(C, k, dtype):
+    """Enough rows that none is split: equal values, few different ones, masked rows, NaN, the largest all in one thread's elements."""
+    from gmk import ops
+    n, some = 520, 14
+    g = torch.Generator().manual_seed(C)
+    x = torch.randn(n, C, generator=torch.Generator("cuda").manual_seed(C), device="cuda")
+    y = _randn(C, some, C)
+    y[0] = 0.0
+    y[1] = -float("inf")
+    y[2] = torch.finfo(torch.float32).min
+    y[3] = torch.randint(0, 3, (C,), generator=g).float()
+    y[4, : C - k // 2] = -float("inf")
+    y[5, ::3] = float("inf")
+    y[6, 5:] = float("nan")
+    y[7, -3:] = float("nan")
+    y[8] = torch.arange(C).float()
+    y[9] = -torch.arange(C).float()
+    y[10, 2048:2052] += 50
+    y[11, ::1024] += 50
+    y[12, C - k:] += 50
+    y[13, 1:] = -float("inf")
+    x[:some] = y.cuda()
+    x = x.to(dtype)
+    v, i = ops.topk_rows(x, k)
+    rows = list(range(some)) + [100, n - 1]
+    _check(x[rows].cpu(), k, (v[rows], i[rows]))
 
 
 @gpu
