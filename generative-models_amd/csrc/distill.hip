@@ -173,9 +173,9 @@ __device__ __forceinline__ float distill_most(const gmk_u32x4& v, float mx) {
 }
 
 // Elements [e, C) of a row from a piece's values, as far as there are any.  `stream`: whole pieces go past the caches, where the logits stay.
-// For the backward pass always (with the loss before it 4096x32768 bf16 193 us, else 207; 8000x8001 fp16 91.6, else 99.8); in one call with
-// the loss, which has no more use for the logits, where rows are whole lines of 128 bytes (4096x32768 bf16 125, else 132; 8000x8001 fp16
-// would take 67, else 61.5).
+// For the backward pass and rows in parts always (with the loss before it 4096x32768 bf16 193 us, else 207; 8000x8001 fp16 91.4, else 99.8;
+// 400x200003 fp16 in parts 100, else 113); for a row in registers, where the logits have no more use, if rows are whole lines of 128 bytes
+// (4096x32768 bf16 125, else 132; 8000x8001 fp16 would take 67, else 61.5).
 template <class T>
 __device__ __forceinline__ void distill_put(T* dzr, int64_t e, int64_t C, const float* o, bool stream) {
   constexpr int VEC = gmk_elem<T>::VEC;
