@@ -19,6 +19,10 @@ __device__ __forceinline__ float4 i8_scaled(const i32x4& v, float xs) {
 __device__ __forceinline__ float4 i8_column(const float4& v, const float4& s, const float4& b) {
   return make_float4(fmaf(v.x, s.x, b.x), fmaf(v.y, s.y, b.y), fmaf(v.z, s.z, b.z), fmaf(v.w, s.w, b.w));
 }
+// a NaN stays one: a row without a scale must not look like a row of zeros
+__device__ __forceinline__ float4 i8_relu(const float4& z) {
+  return make_float4(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y, z.z < 0.f ? 0.f : z.z, z.w < 0.f ? 0.f : z.w);
+}
 template <class T>
 __device__ __forceinline__ void i8_put4(const float4& z, T* p, int have) {   // the first `have` of 4 columns
   T t[4] = {(T)z.x, (T)z.y, (T)z.z, (T)z.w};
@@ -274,7 +278,7 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
           }
         } else if (act == GMK_ACT_RELU) {
 #pragma unroll
-          for (int u = 0; u < 16 / STEP; ++u) z[u] = make_float4(z[u].x > 0.f ? z[u].x : 0.f, z[u].y > 0.f ? z[u].y : 0.f, z[u].z > 0.f ? z[u].z : 0.f, z[u].w > 0.f ? z[u].w : 0.f);
+          for (int u = 0; u < 16 / STEP; ++u) z[u] = i8_relu(z[u]);
         }
         T* const yq = y + (int64_t)(mb + q0) * N + n;
         if (whole && lines) {
@@ -450,7 +454,8 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_i8_rows_kernel(const X* __res
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) v += part[w * NT * 64 + q];
     float4 z = i8_column(i8_scaled(v, xs), cs, cb), d;
-    GMK_WITH_ACT(act, [&](auto f) { float4 a; f(z, a, d); z = a; });
+    if (act == GMK_ACT_RELU) z = i8_relu(z);
+    else GMK_WITH_ACT(act, [&](auto f) { float4 a; f(z, a, d); z = a; });
     i8_put4<T>(z, y + (int64_t)m * N + n, N - n);
   }
 }

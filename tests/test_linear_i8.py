@@ -194,6 +194,18 @@ def test_linear_i8_rows_are_independent_and_nan_stays_in_its_row(M):
 
 
 @gpu
+@pytest.mark.parametrize("act", [None, "relu", "leaky-relu", "elu", "selu", "gelu", "swish", "mish", "sigmoid"])
+@pytest.mark.parametrize("M,N", [(1, 33), (3, 9000), (9, 40), (33, 2050), (300, 1100), (1100, 3101)])
+def test_linear_i8_keeps_nan_behind_every_activation(M, N, act):
+    from gmk import ops
+    x = _randn(5, M, 100)
+    x[M // 2, 7] = float("nan")
+    wq, ws = ops.quantize_rows(_randn(6, N, 100).cuda())
+    nan = torch.isnan(ops.linear_i8(x.cuda(), wq, ws, act=act))
+    assert nan[M // 2].all() and nan.sum() == N
+
+
+@gpu
 @pytest.mark.parametrize("act", ["leaky-relu", "elu", "selu", "swish", "mish", "sigmoid"])
 def test_linear_i8_activations(act):
     """Every activation of the fp32 layer, on the same values: linear_fwd with the identity as its weight applies it in fp32."""
