@@ -339,7 +339,7 @@ int gmk_quantize_rows(const void* x, int xtype, signed char* q, float* scale, in
 
 /* gmk_gemm_i8: y (M,N) = act((sum_k xq[m][k] wq[n][k]) * xscale[m] * wscale[n] + bias[n]), the sum exact in 32-bit
  *   integers.  xq (M,K), wq (N,K) int8 in [-128, 127], K % 16 == 0 (rows that gmk_quantize_rows padded are whole), K <= GMK_I8_MAX_K,
- *   M and N <= GMK_I8_MAX_ROWS; bias (N) fp32 or NULL; act: enum gmk_act (each keeps a NaN). */
+ *   M and N <= GMK_I8_MAX_ROWS; bias (N) fp32 or NULL; act: enum gmk_act, each of which keeps a NaN. */
 #define GMK_I8_MAX_K 131056
 #define GMK_I8_MAX_ROWS (1 << 30) /* M and N */
 int gmk_gemm_i8(const signed char* xq, const float* xscale, const signed char* wq, const float* wscale, const float* bias,
