@@ -170,6 +170,8 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));   // what the scales and the epilogue derive from it is derived there, not kept in registers
     const unsigned to = __builtin_amdgcn_readfirstlane(gmk_lds_addr(part));
+    // the epilogue before this one is done with the part: a load to LDS waits for no LDS operation that is still out
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     auto one = [&](const float* from, int have, int most, int at) {
       const i32x4 rs = i8_buffer(from, min(max(have, 0), most) * 4);
 #pragma unroll
@@ -257,11 +259,11 @@ __global__ __launch_bounds__(64 * WGN * WGM, 2) void gemm_i8_tile_kernel(const s
     const bool lines = (((uintptr_t)y | (uintptr_t)((int64_t)N * sizeof(T))) & 127) == 0;
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
+      const int mb = m0 + wm + 16 * j;
+      if (mb >= M) break;   // before the sums are written: what a wave writes to its part it also reads
 #pragma unroll
       for (int i = 0; i < TN; ++i) *(float4*)(part + r * LD + (((4 * i + kq) ^ r) & (PER_ROW - 1)) * 4) = i8_scaled(acc[i][j], xs[j]);
       __builtin_amdgcn_wave_barrier();
-      const int mb = m0 + wm + 16 * j;
-      if (mb >= M) break;
       if (common) {
         float4 z[16 / STEP];
 #pragma unroll

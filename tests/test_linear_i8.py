@@ -161,6 +161,22 @@ def test_gemm_i8_larger_kernels(shape):
         assert ((y - r).abs() <= tol).all(), act
 
 
+# M ends so early inside the last tile that some of its waves have no row, and a workgroup takes another tile behind one of those (more tiles
+# than run at once on 256 compute units): 64x32, 64x64, 128x192, 128x128 and 256x256
+@gpu
+@pytest.mark.parametrize("shape", [(10, 256, 40000), (36, 1920, 32960), (528, 896, 26304), (263, 128, 34688), (649, 128, 33536), (649, 144, 33533)])
+def test_gemm_i8_next_tile_has_its_own_scales(shape):
+    """Sums below 2^24 and scales that are powers of two: every output is exact, and one with another tile's scales is not."""
+    from gmk import ops
+    M, K, N = shape
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    xq, wq = (torch.randint(-60, 61, (n, K), generator=g, device="cuda").to(torch.int8) for n in (M, N))
+    xs, ws = (2.0 ** torch.randint(-8, 9, (n,), generator=g, device="cuda") for n in (M, N))
+    ref = (xq.double() @ wq.double().t().contiguous()) * xs.double()[:, None] * ws.double()
+    for _ in range(3):
+        assert torch.equal(ops.matmul_i8(xq, xs, wq, ws).double(), ref)
+
+
 @gpu
 @pytest.mark.parametrize("dtype,M,K,N", [(torch.bfloat16, 9001, 4100, 130), (torch.float32, 4500, 4097, 300), (torch.float16, 700, 8200, 12000)])
 def test_linear_i8_large_is_its_two_steps(dtype, M, K, N):
