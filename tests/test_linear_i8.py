@@ -161,6 +161,54 @@ def test_gemm_i8_larger_kernels(shape):
         assert ((y - r).abs() <= tol).all(), act
 
 
+def _kernels(call):
+    """The template arguments behind the type, of every 8-bit product that `call` launches: "64, 32, 2, 2, 6" (columns and rows of a tile, waves
+    both ways, stages)."""
+    torch.cuda.synchronize()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        call()
+        torch.cuda.synchronize()
+    return [e.name.split("<")[1].split(">")[0].split(", ", 1)[1] for e in prof.events() if "gemm_i8_tile_kernel<" in e.name]
+
+
+# Whole lines of y (N a multiple of 64: stores past the caches in every type), whole chunks of K (a multiple of 128) and M that ends inside a
+# tile, for every tile shape above 32x32: with one tile a workgroup, and with several, whose loads run over from one tile into the next.
+# The kernel that each size is here for is checked by name, so that another choice of kernels cannot leave one out.
+WHOLE_LINES = [("64, 32, 2, 2, 6", (30, 1024, 17024)), ("64, 32, 2, 2, 6", (24, 256, 40000)), ("64, 64, 2, 2, 4", (36, 1920, 32960)),
+               ("128, 128, 4, 2, 4", (65, 1024, 17024)), ("128, 128, 4, 2, 4", (1100, 1280, 3136)), ("128, 192, 4, 2, 3", (777, 1408, 5056)),
+               ("128, 192, 4, 2, 3", (528, 896, 26304)), ("128, 128, 2, 2, 2", (1500, 1408, 5056)), ("128, 128, 2, 2, 2", (263, 128, 34688)),
+               ("256, 256, 4, 2, 2", (4090, 2048, 4096)), ("256, 256, 4, 2, 2", (8100, 1024, 8256)), ("256, 256, 4, 2, 2", (649, 128, 33536))]
+
+
+@gpu
+@pytest.mark.parametrize("kernel,shape", WHOLE_LINES)
+def test_gemm_i8_whole_lines_and_chunks(kernel, shape):
+    """As test_gemm_i8_larger_kernels: exact whole numbers in fp32, then scales, bias and activation in each type."""
+    from gmk import ops
+    M, K, N = shape
+    assert N % 64 == 0 and K % 128 == 0
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    xq, wq = (torch.randint(-60, 61, (n, K), generator=g, device="cuda").to(torch.int8) for n in (M, N))
+    one = torch.ones(max(M, N), device="cuda")
+    ref = xq.double() @ wq.double().t().contiguous()
+    got = []
+    ran = _kernels(lambda: got.append(ops.matmul_i8(xq, one[:M].contiguous(), wq, one[:N].contiguous())))
+    assert got[0].data_ptr() % 128 == 0
+    assert torch.equal(got[0].double(), ref)
+    xs, ws, b = (torch.rand(n, generator=g, device="cuda") + 0.5 for n in (M, N, N))
+    xs = xs / K
+    for act, dtype in ((None, torch.bfloat16), ("relu", torch.bfloat16), ("gelu", torch.float16), ("elu", torch.float32)):
+        y = ops.matmul_i8(xq, xs, wq, ws, b, act=act, out_dtype=dtype).double()
+        z = ref * xs.double()[:, None] * ws.double() + b.double()
+        r = _act(act, z)
+        tol = (z.abs() + 2 * b.double()) * (4 * 2.0 ** -24 * 1.13 + 1.5e-7 + 8 * 2.0 ** -24)   # as in test_linear_i8
+        tol += torch.finfo(dtype).eps / 2 * (r.abs() + tol) + (2.0 ** -25 if dtype == torch.float16 else 0)
+        assert ((y - r).abs() <= tol).all(), act
+    if not ran:
+        pytest.skip("the results are right, but the profiler names no kernel here")
+    assert ran == [kernel]
+
+
 # M ends so early inside the last tile that some of its waves have no row, and a workgroup takes another tile behind one of those (more tiles
 # than run at once on 256 compute units): 64x32, 64x64, 128x192, 128x128 and 256x256
 @gpu
