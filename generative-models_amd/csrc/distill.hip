@@ -107,6 +107,11 @@ struct DistillGrad {
   template <class T>
   __device__ __forceinline__ void piece(const DistillArgs& a, const gmk_u32x4& v, float* o) const {
     constexpr int VEC = gmk_elem<T>::VEC;
+    if (gt == 0.f && g1 == 0.f) {   // a row with neither part gives zeros, whatever its logits are: NaN * 0 is none
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[i] = 0.f;
+      return;
+    }
     float d[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) d[i] = gmk_piece<T>(v, i) - mx;

@@ -366,7 +366,8 @@ int gmk_topk_rows(const void* x, int xtype, void* value, int* index, int64_t n, 
  *     loss = soft T^2 sum_j p_j (ln p_j - ln q_{idx_j}) + hard (-ln softmax(z)_label),
  *     d loss / d z_c = soft T (q_c - p_c) + hard (softmax(z)_c - [c = label]).
  *   An idx outside [0, C) is no entry, and a row without an entry of a weight above 0 has no soft part; a label outside [0, C)
- *   (say -100) or labels == NULL: no hard part.  A row whose logits are all -inf gives loss 0 and gradient 0.  The same class may be
+ *   (say -100) or labels == NULL: no hard part.  A row with neither part gives loss 0 and gradient 0 whatever its logits hold, and so does one
+ *   whose logits are all -inf.  The same class may be
  *   listed more than once.  The soft loss is a difference of sums in 32 bits, known to about soft T^2 2^-20: at temperatures far above the
  *   logits' differences it loses its digits (the gradient does not).  z and dz share ztype, t has ttype.  1 <= k <= GMK_DISTILL_MAX_K, C < 2^31, T between 2^-60 and 2^60.
  * gmk_distill_fwd: loss (n) fp32 and stats (n,3) fp32 (the row's maximum and its two sums of exponentials) for the backward pass.

@@ -185,6 +185,43 @@ def test_distill_padding_rows_and_nan(C):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [10, 3001, 40000, 100000])
+def test_distill_rows_with_nothing_to_learn(C, dtype):
+    """No entry and no label: loss 0 and gradient 0 at a weight of 1, whatever the logits hold (an ignored sample of a batch); a row with one
+    of the two parts still shows them."""
+    from gmk import ops
+    from models.classifiers import distillation_loss
+    z, t, idx, labels = (v.cuda() for v in _case(C + 1, 9, C, 4, dtype, pads=False))
+    clean = ops.distill_fwd_bwd(z, t, idx, labels, 2.0, 1.0, 0.5)
+    idx[[1, 3, 5, 7]], labels[[1, 3, 5, 7]] = -1, -100
+    z[1] = math.nan
+    z[3, C // 2] = math.nan
+    z[5, C - 1] = math.inf
+    z[7] = math.inf
+    idx[4], z[4, C // 3] = -1, math.nan         # a label is left
+    labels[6], z[6, C // 3] = -100, math.nan    # entries are left
+    none, bad, others = [1, 3, 5, 7], [4, 6], [0, 2, 8]
+    one = torch.ones(9, device="cuda")
+    for weight in (None, one):
+        l, g = ops.distill_fwd_bwd(z, t, idx, labels, 2.0, 1.0, 0.5, weight)
+        assert not l[none].any() and not g[none].any()
+        assert torch.isnan(l[bad]).all() and torch.isnan(g[bad]).all()
+        assert torch.equal(l[others], clean[0][others]) and torch.equal(g[others], clean[1][others])
+    l, stats = ops.distill_fwd(z, t, idx, labels, 2.0, 1.0, 0.5)
+    g = ops.distill_bwd(one, z, t, idx, labels, stats, 2.0, 1.0, 0.5)
+    assert not l[none].any() and not g[none].any() and torch.isnan(g[bad]).all() and torch.isfinite(g[others]).all()
+    # parts that are switched off by their weight; through autograd, whose mean the ignored samples leave as it is
+    for soft, hard, row in ((0.0, 0.5, 6), (1.0, 0.0, 4)):
+        l, g = ops.distill_fwd_bwd(z, t, idx, labels, 2.0, soft, hard)
+        assert not l[none + [row]].any() and not g[none + [row]].any()
+    live = others + none
+    a = z[live].clone().requires_grad_(True)
+    distillation_loss(a, t[live], idx[live], labels[live], 2.0, 1.0, 0.5).mean().backward()
+    assert torch.isfinite(a.grad).all() and a.grad[:3].any() and not a.grad[3:].any()
+
+
+@gpu
 def test_distill_gradient_against_differences():
     """Central differences of the loss itself.  Step h = 2^-6: the loss' third derivative is at most soft / T + hard <= 1.25 and its
     error about 1e-6, so that the quotient is off by h^2 / 6 * 1.25 + 1e-6 / h < 2e-4."""
