@@ -544,7 +544,8 @@ def softmax_stats(logits, out=None, topn=3, eps=1e-7):
 
 # ---- a classifier made smaller: 8-bit linear layers, the k largest logits, distillation from them ----------------------------
 # These take fp32, bf16 or fp16 tensors.  Their scratch is a tensor of the call's own, from torch's allocator: calls on different
-# streams and captured graphs share none of it.
+# streams and captured graphs share none of it.  Under a handle that is not torch's current stream (SideQueue.run) the allocator is told
+# that the scratch is in use there; what such a call returns is the caller's to keep until join(), as with every other op.
 _FLOAT_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FP32, _INT8, _INT32, _INT64 = (torch.float32,), (torch.int8,), (torch.int32,), (torch.int64,)
 I8_MAX_K, TOPK_MAX, DISTILL_MAX_K = 131056, 256, 256   # include/gmk.h
@@ -594,7 +595,12 @@ def _scratch_bytes(name, *sizes):
 def _scratch(device, name, *sizes):
     """(tensor or None, its bytes) of the scratch that an entry point asks for."""
     nbytes = _scratch_bytes(name, *sizes)
-    return (_new_rows(nbytes, 0, device, torch.uint8), nbytes) if nbytes else (None, 0)
+    if not nbytes:
+        return None, 0
+    t = _new_rows(nbytes, 0, device, torch.uint8)
+    if _cur_stream is not None and _cur_stream != torch._C._cuda_getCurrentRawStream(t.get_device()):
+        t.record_stream(torch.cuda.ExternalStream(_cur_stream, device=device))
+    return t, nbytes
 
 
 def quantize_rows(x):

@@ -145,6 +145,34 @@ def test_topk_rows_streams_graphs_and_empty():
     assert v.shape == i.shape == (0, 5)
 
 
+@gpu
+def test_scratch_under_another_stream_handle(monkeypatch):
+    """Calls in SideQueue.run, where the launch goes to a side stream and torch's current stream stays: the scratch that dies with the call
+    is not handed out again while the side stream, held up by a wait of some milliseconds, has yet to use it."""
+    from gmk import ops
+    x = _randn(1, 3, 90001).cuda()
+    ref = ops.topk_rows(x, 40)
+    seen = []
+    real = ops._scratch
+    monkeypatch.setattr(ops, "_scratch", lambda *a: [seen.append((t.data_ptr(), b)) or (t, b) for t, b in [real(*a)]][0])
+    kept = ops.topk_rows(x, 40)
+    again = torch.empty(seen[-1][1], dtype=torch.uint8, device="cuda")
+    assert again.data_ptr() == seen[-1][0]   # a call on the current stream: its scratch is free behind it, in the stream's order
+    del again, kept
+    torch.cuda.synchronize()
+    side = ops.SideQueue(x.device)
+    for st in side.streams:
+        with torch.cuda.stream(st):
+            torch.cuda._sleep(20_000_000)
+    out = side.run(lambda: ops.topk_rows(x, 40), x)
+    others = [torch.full((seen[-1][1],), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    at, size = seen[-1]
+    assert all(o.data_ptr() >= at + size or o.data_ptr() + size <= at for o in others)
+    side.join()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+
+
 def test_topk_rows_refusals():
     from gmk import lib, ops
     h = lib()
