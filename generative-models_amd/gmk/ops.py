@@ -548,7 +548,7 @@ def softmax_stats(logits, out=None, topn=3, eps=1e-7):
 # that the scratch is in use there; what such a call returns is the caller's to keep until join(), as with every other op.
 _FLOAT_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FP32, _INT8, _INT32, _INT64 = (torch.float32,), (torch.int8,), (torch.int32,), (torch.int64,)
-I8_MAX_K, TOPK_MAX, DISTILL_MAX_K = 131056, 256, 256   # include/gmk.h
+I8_MAX_K, I8_MAX_ROWS, TOPK_MAX, DISTILL_MAX_K = 131056, 1 << 30, 256, 256   # include/gmk.h
 
 
 def _chk_rows(name, t, dtypes, shape, dev):
@@ -608,8 +608,8 @@ def quantize_rows(x):
     Weights (rows = output channels) are quantised by it once, activations by linear_i8 in every call."""
     dev = _chk_first("x", x, _FLOAT_IDS)
     M, K = x.shape
-    if K == 0:
-        raise ValueError("x must have at least one column")
+    if not 1 <= K <= I8_MAX_ROWS:   # both sizes are C ints
+        raise ValueError(f"x must have 1 to {I8_MAX_ROWS} columns, not {K}")
     ld = -(-K // 16) * 16
     q = _new_rows(M, ld, x.device, torch.int8)
     scale = _new_rows(M, 0, x.device, torch.float32)
@@ -617,13 +617,15 @@ def quantize_rows(x):
     return q, scale
 
 
-def _i8_args(dev, K, wq, wscale, bias, out_dtype):
+def _i8_args(dev, M, K, wq, wscale, bias, out_dtype):
     if out_dtype not in _FLOAT_IDS:
         raise ValueError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
     if K == 0 or K > I8_MAX_K:
         raise ValueError(f"the 8-bit product takes 1 to {I8_MAX_K} columns, not {K}")
     _chk_rows("wq", wq, _INT8, None, dev)
     N, ld = wq.shape
+    if M > I8_MAX_ROWS or N > I8_MAX_ROWS:   # C ints: more of them would arrive there cut to 32 bits
+        raise ValueError(f"the 8-bit product takes up to {I8_MAX_ROWS} rows on either side, not {M} and {N}")
     if N == 0 or ld != -(-K // 16) * 16:
         raise ValueError(f"wq must have at least one row and {-(-K // 16) * 16} columns ({K} rounded up to 16), not {tuple(wq.shape)}")
     _chk_rows("wscale", wscale, _FP32, (N,), dev)
@@ -639,7 +641,7 @@ def matmul_i8(xq, xscale, wq, wscale, bias=None, act=None, out_dtype=torch.float
     if K % 16:
         raise ValueError(f"xq has {K} columns: rows of 8-bit values are padded to a multiple of 16 (quantize_rows)")
     _chk_rows("xscale", xscale, _FP32, (M,), dev)
-    N = _i8_args(dev, K, wq, wscale, bias, out_dtype)
+    N = _i8_args(dev, M, K, wq, wscale, bias, out_dtype)
     y = _new_rows(M, N, xq.device, out_dtype)
     check(lib().gmk_gemm_i8(_p(xq), _p(xscale), _p(wq), _p(wscale), _p(bias), _p(y), _FLOAT_IDS[out_dtype], M, K, N, act_id(act),
                             _stream_of(dev)))
@@ -652,7 +654,7 @@ def linear_i8(x, wq, wscale, bias=None, act=None, out_dtype=None):
     dev = _chk_first("x", x, _FLOAT_IDS)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     M, K = x.shape
-    N = _i8_args(dev, K, wq, wscale, bias, out_dtype)
+    N = _i8_args(dev, M, K, wq, wscale, bias, out_dtype)
     y = _new_rows(M, N, x.device, out_dtype)
     ws, nbytes = _scratch(x.device, "gmk_linear_i8_workspace_bytes", M, K, N)
     check(lib().gmk_linear_i8_fwd(_p(x), _FLOAT_IDS[x.dtype], _p(wq), _p(wscale), _p(bias), _p(y), _FLOAT_IDS[out_dtype], M, K, N,

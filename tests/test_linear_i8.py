@@ -349,6 +349,25 @@ def test_wrappers_refuse_cpu_tensors():
             call()
 
 
+def test_wrappers_refuse_sizes_beyond_32_bits(monkeypatch):
+    """Rows and columns that a C int would cut (2^32 + 5 rows to 5, with the others never written), on tensors without memory."""
+    from gmk import ops
+    monkeypatch.setattr(ops, "_chk_first", lambda *a: 0)
+    monkeypatch.setattr(ops, "_chk_rows", lambda *a: None)
+
+    def calls(M, K, N):
+        x, q, w = (torch.empty(n, c, dtype=d, device="meta") for n, c, d in ((M, K, torch.bfloat16), (M, K, torch.int8), (N, K, torch.int8)))
+        return (lambda: ops.linear_i8(x, w, None)), (lambda: ops.matmul_i8(q, None, w, None))
+
+    for M, N in (((1 << 32) + 5, 7), (7, (1 << 32) + 5), ((1 << 30) + 1, 7), (7, (1 << 30) + 1)):
+        for call in calls(M, 16, N):
+            with pytest.raises(ValueError, match="rows"):
+                call()
+    for K in ((1 << 32) + 16, (1 << 30) + 16):
+        with pytest.raises(ValueError, match="columns"):
+            ops.quantize_rows(torch.empty(1, K, device="meta"))
+
+
 def test_c_entries_refuse_bad_arguments():
     """Every check comes before the first launch, so that it can be made without a GPU."""
     from gmk import lib
