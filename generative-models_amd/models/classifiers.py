@@ -62,7 +62,7 @@ class Classifier(nn.Module):
                 w = layer.weight * s.view(-1, *([1] * (layer.weight.dim() - 1)))
                 b = (layer.bias - bn.running_mean) * s + bn.bias
                 out[layer] = (w.float().contiguous(), b.float().contiguous())
-            out[self.fc_out] = (self.fc_out.weight.detach().float().contiguous(), self.fc_out.bias.detach().float().contiguous())
+            out[self.fc_out] = (self.fc_out.weight.detach(), self.fc_out.bias.detach())   # as they are: other types are refused by the ops
             if self.int8_fc:
                 for layer in (self.fc, self.fc_out):
                     w, b = out[layer]

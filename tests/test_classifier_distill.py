@@ -84,6 +84,27 @@ def test_int8_layers_follow_replaced_weights():
     assert torch.equal(m(x), fresh(x))
 
 
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16])
+def test_output_layer_of_another_type_is_not_cast(dtype):
+    """fc_out has no BatchNorm to be folded with: its tensors reach the ops as they are, which refuse another type than fp32."""
+    m, _ = _classifier()
+    m.fc_out.to(dtype)
+    w, b = m.eval()._folded()[m.fc_out]
+    assert w.dtype == b.dtype == dtype and w.data_ptr() == m.fc_out.weight.data_ptr()
+
+
+@gpu
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16])
+def test_output_layer_of_another_type_is_refused(dtype, int8):
+    m, _ = _classifier()
+    m = m.cuda().eval()
+    m.fc_out.to(dtype)
+    m.int8_fc = int8
+    with pytest.raises(ValueError):
+        m(torch.rand(4, 3, 32, 32).cuda())
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_distillation_loss_gradient(dtype):
