@@ -49,12 +49,21 @@ class Classifier(nn.Module):
     def _folded(self):
         """BatchNorm (eval: running statistics) folded into the producing layer:
         bn(conv(x)) = conv(x; w * s) + (b - mean) * s + beta,  s = gamma / sqrt(var + eps).
-        Cached until a parameter or buffer is modified in place (tensor version counters) or replaced."""
+        Cached until a parameter or buffer is modified in place (tensor version counters) or replaced.  A graph that is being captured folds for
+        itself: its replays follow the weights, and neither uses what the other frees or has yet to compute."""
+        if self.fc_out.weight.is_cuda and torch.cuda.is_current_stream_capturing():
+            return self._fold()
         tensors = list(self.parameters()) + list(self.buffers())
         key = (self.int8_fc,) + tuple((t.data_ptr(), t._version) for t in tensors)
         cache = self.__dict__.get("_gmk_fold")
         if cache is not None and cache[0] == key:
             return cache[1]
+        out = self._fold()
+        # the tensors themselves are kept too: memory that a later weight could be given is no key
+        self.__dict__["_gmk_fold"] = (key, out, [t.detach() for t in tensors])
+        return out
+
+    def _fold(self):
         out = {}
         with torch.no_grad():
             for layer, bn in ((self.conv1, self.bn1), (self.conv2, self.bn2), (self.conv3, self.bn3), (self.fc, self.bn4)):
@@ -67,8 +76,6 @@ class Classifier(nn.Module):
                 for layer in (self.fc, self.fc_out):
                     w, b = out[layer]
                     out[layer] = (*ops.quantize_rows(w), b)
-        # the tensors themselves are kept too: memory that a later weight could be given is no key
-        self.__dict__["_gmk_fold"] = (key, out, [t.detach() for t in tensors])
         return out
 
     def _forward_gmk(self, x):

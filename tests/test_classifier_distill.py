@@ -84,6 +84,41 @@ def test_int8_layers_follow_replaced_weights():
     assert torch.equal(m(x), fresh(x))
 
 
+@gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_classifier_in_a_graph(int8):
+    """The eval forward captured before it ever ran: an eager call ahead of the first replay has weights of its own, and replays follow the
+    weights as they are updated, with eager work between them."""
+    def fresh(of):
+        other, _ = _classifier()
+        other = other.cuda().eval()
+        other.load_state_dict(of.state_dict())
+        other.int8_fc = int8
+        return other
+
+    m, _ = _classifier(3)
+    m = m.cuda().eval()
+    m.int8_fc = int8
+    static, x = (torch.rand(16, 3, 32, 32, generator=torch.Generator().manual_seed(i)).cuda() for i in range(2))
+    fresh(m)(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(g):
+        y = m(static)
+    assert torch.equal(m(x), fresh(m)(x))
+    for i in range(3):
+        with torch.no_grad():
+            m.fc.weight.mul_(1.25)
+            m.fc_out.weight.add_(0.125)
+            m.bn1.running_mean.add_(0.25)
+            static.copy_(torch.rand(16, 3, 32, 32, generator=torch.Generator().manual_seed(10 + i)))
+        junk = [torch.full((1 << 20,), 1e30, device="cuda") for _ in range(8)]   # into whatever the eager calls have let go of
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, fresh(m)(static)) and torch.equal(m(x), fresh(m)(x))
+        del junk
+
+
 @pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16])
 def test_output_layer_of_another_type_is_not_cast(dtype):
     """fc_out has no BatchNorm to be folded with: its tensors reach the ops as they are, which refuse another type than fp32."""
