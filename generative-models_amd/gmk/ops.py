@@ -64,6 +64,12 @@ def _new_like(x):
     return t
 
 
+def keep_recorded(*tensors):
+    """Tensors that a caller made and hands to these wrappers: a launch plan that is being recorded keeps them too."""
+    if _rec_keep is not None:
+        _rec_keep.extend(tensors)
+
+
 def _chk(*ts):
     for t in ts:
         if t is None:

@@ -57,6 +57,7 @@ class Classifier(nn.Module):
         key = (self.int8_fc,) + tuple((t.data_ptr(), t._version) for t in tensors)
         cache = self.__dict__.get("_gmk_fold")
         if cache is not None and cache[0] == key:
+            ops.keep_recorded(*(t for layer in cache[1].values() for t in layer))
             return cache[1]
         out = self._fold()
         # the tensors themselves are kept too: memory that a later weight could be given is no key
@@ -72,6 +73,7 @@ class Classifier(nn.Module):
                 b = (layer.bias - bn.running_mean) * s + bn.bias
                 out[layer] = (w.float().contiguous(), b.float().contiguous())
             out[self.fc_out] = (self.fc_out.weight.detach(), self.fc_out.bias.detach())   # as they are: other types are refused by the ops
+            ops.keep_recorded(*(t for layer in out.values() for t in layer))
             if self.int8_fc:
                 for layer in (self.fc, self.fc_out):
                     w, b = out[layer]

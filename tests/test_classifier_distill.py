@@ -119,6 +119,44 @@ def test_classifier_in_a_graph(int8):
         del junk
 
 
+@gpu
+@pytest.mark.parametrize("warm", [False, True])
+@pytest.mark.parametrize("int8", [False, True])
+def test_classifier_in_a_launch_plan(int8, warm):
+    """A recorded eval forward owns the folded weights that it names: replays answer with those of the recording, whatever became of the
+    classifier's own since."""
+    from gmk.plan import StepPlan
+    m, _ = _classifier(3)
+    m = m.cuda().eval()
+    m.int8_fc = int8
+    xs = [torch.rand(16, 3, 32, 32, generator=torch.Generator().manual_seed(i)).cuda() for i in range(3)]
+    other, _ = _classifier()
+    other = other.cuda().eval()
+    other.load_state_dict(m.state_dict())
+    other.int8_fc = int8
+    want = [other(x).clone() for x in xs]
+    if warm:
+        m(xs[0])
+    with torch.no_grad(), StepPlan() as plan:
+        y = m(xs[0])
+    plan.set_inputs(xs[0])
+    assert torch.equal(y, want[0])
+    with torch.no_grad():
+        for name, p in m.named_parameters():
+            if not name.startswith("fc_out"):   # whose weight is the parameter itself, and part of no fold
+                p.mul_(3.0)
+    m.bn1.running_mean.add_(1.0)
+    m(xs[0])
+    torch.cuda.synchronize()
+    junk = [torch.full((n,), 1e30, device="cuda") for n in (10, 64, 128, 256, 640, 4800, 204800, 262144, 294912) for _ in range(4)]
+    for i in (1, 2, 0):
+        plan.enqueue(0, plan.nseg, xs[i])
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i])
+    del junk
+    plan.close()
+
+
 @pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16])
 def test_output_layer_of_another_type_is_not_cast(dtype):
     """fc_out has no BatchNorm to be folded with: its tensors reach the ops as they are, which refuse another type than fp32."""
