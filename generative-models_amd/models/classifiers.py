@@ -55,14 +55,17 @@ class Classifier(nn.Module):
             return self._fold()
         tensors = list(self.parameters()) + list(self.buffers())
         key = (self.int8_fc,) + tuple((t.data_ptr(), t._version) for t in tensors)
+        # a fold for each stream that asks: what one of them has only queued is no weight for the others
+        stream = torch._C._cuda_getCurrentRawStream(tensors[0].get_device()) if tensors[0].is_cuda else None
         cache = self.__dict__.get("_gmk_fold")
-        if cache is not None and cache[0] == key:
-            ops.keep_recorded(*(t for layer in cache[1].values() for t in layer))
-            return cache[1]
-        out = self._fold()
-        # the tensors themselves are kept too: memory that a later weight could be given is no key
-        self.__dict__["_gmk_fold"] = (key, out, [t.detach() for t in tensors])
-        return out
+        if cache is None or cache[0] != key:
+            # the tensors themselves are kept too: memory that a later weight could be given is no key
+            cache = self.__dict__["_gmk_fold"] = (key, {}, [t.detach() for t in tensors])
+        if stream in cache[1]:
+            ops.keep_recorded(*(t for layer in cache[1][stream].values() for t in layer))
+        else:
+            cache[1][stream] = self._fold()
+        return cache[1][stream]
 
     def _fold(self):
         out = {}

@@ -120,6 +120,45 @@ def test_classifier_in_a_graph(int8):
 
 
 @gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_classifier_on_two_streams(monkeypatch, int8):
+    """The first forward on a stream that is held up for some milliseconds, the next on another one: it does not use what the first has only
+    queued.  Each stream folds once for all its calls, and again after an update."""
+    from models.classifiers import Classifier
+    m, _ = _classifier(3)
+    m = m.cuda().eval()
+    m.int8_fc = int8
+    xs = [torch.rand(16, 3, 32, 32, generator=torch.Generator().manual_seed(i)).cuda() for i in range(2)]
+    other, _ = _classifier()
+    other = other.cuda().eval()
+    other.load_state_dict(m.state_dict())
+    other.int8_fc = int8
+    want = [other(x).clone() for x in xs]
+    folds = []
+    real = Classifier._fold
+    monkeypatch.setattr(Classifier, "_fold", lambda self: folds.append(1) or real(self))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(3):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            torch.cuda._sleep(20_000_000)
+        got = []
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(m(x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+        assert len(folds) == 2
+    with torch.no_grad():
+        m.fc.bias.add_(0.0)
+    torch.cuda.synchronize()
+    for s, x, w in zip(streams, xs, want):
+        with torch.cuda.stream(s):
+            assert torch.equal(m(x), w)
+    assert len(folds) == 4
+
+
+@gpu
 @pytest.mark.parametrize("warm", [False, True])
 @pytest.mark.parametrize("int8", [False, True])
 def test_classifier_in_a_launch_plan(int8, warm):
