@@ -49,7 +49,8 @@ class Classifier(nn.Module):
     def _folded(self):
         """BatchNorm (eval: running statistics) folded into the producing layer:
         bn(conv(x)) = conv(x; w * s) + (b - mean) * s + beta,  s = gamma / sqrt(var + eps).
-        Cached until a parameter or buffer is modified in place (tensor version counters) or replaced.  A graph that is being captured folds for
+        Cached until a parameter or buffer is modified in place (tensor version counters) or replaced, the classifier is moved or goes into
+        train mode.  A graph that is being captured folds for
         itself: its replays follow the weights, and neither uses what the other frees or has yet to compute."""
         if self.fc_out.weight.is_cuda and torch.cuda.is_current_stream_capturing():
             return self._fold()
@@ -66,6 +67,16 @@ class Classifier(nn.Module):
         else:
             cache[1][stream] = self._fold()
         return cache[1][stream]
+
+    def train(self, mode=True):
+        # training may write parameters where no version counter sees it: optimizers on raw pointers (gmk.optim), replayed graphs
+        if mode:
+            self.__dict__.pop("_gmk_fold", None)
+        return super().train(mode)
+
+    def _apply(self, *args, **kwargs):
+        self.__dict__.pop("_gmk_fold", None)   # or a model that moves would leave its memory behind
+        return super()._apply(*args, **kwargs)
 
     def _fold(self):
         out = {}

@@ -119,6 +119,47 @@ def test_classifier_in_a_graph(int8):
         del junk
 
 
+def test_folded_weights_go_with_training_and_moving():
+    """Updates that no version counter shows (here through numpy's view of the memory) between two eval phases, and a move: the eval forward
+    folds again, and nothing holds the old tensors."""
+    m, _ = _classifier()
+    m.eval()
+    before = m._folded()[m.fc][0].clone()
+    assert m._folded()[m.fc][0] is m._folded()[m.fc][0]
+    m.train()
+    m.fc.weight.detach().numpy()[:] *= 2
+    m.eval()
+    assert torch.equal(m._folded()[m.fc][0], 2 * before)
+    m.eval()
+    assert "_gmk_fold" in m.__dict__   # a call of eval() alone costs no fold
+    m.to(torch.float64)
+    assert "_gmk_fold" not in m.__dict__
+
+
+@gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_classifier_after_training_with_the_fused_optimizer(int8):
+    """FusedAdamW writes the parameters on raw pointers; the backward pass is made up, so that no forward touches the version counters either."""
+    from gmk.optim import FusedAdamW
+    m, _ = _classifier()
+    m = m.cuda()
+    m.int8_fc = int8
+    x = torch.rand(8, 3, 32, 32, generator=torch.Generator().manual_seed(5)).cuda()
+    optim = FusedAdamW(m.parameters(), lr=0.05, weight_decay=0.0)
+    first = m.eval()(x).clone()
+    for turn in range(2):
+        m.train()
+        optim.zero_grad()
+        optim.flat_grad.copy_(torch.randn(optim.flat_grad.shape, generator=torch.Generator().manual_seed(turn)))
+        optim.step()
+        y = m.eval()(x)
+        fresh, _ = _classifier()
+        fresh.load_state_dict(m.state_dict())
+        fresh = fresh.cuda().eval()
+        fresh.int8_fc = int8
+        assert torch.equal(y, fresh(x)) and not torch.equal(y, first)
+
+
 @gpu
 @pytest.mark.parametrize("int8", [False, True])
 def test_classifier_on_two_streams(monkeypatch, int8):
