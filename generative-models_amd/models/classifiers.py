@@ -185,7 +185,7 @@ def _epoch_accuracy(classifier, dataloader, device, step=None):
 def train_classifier(args, classifier=None, train_dataloader=None, test_dataloader=None, device=None, teacher=None):
     """Auxiliary model training (reference classifiers.py:77-113): cross entropy, AdamW, cosine LR stepped every
     iteration over epochs * len(loader) steps; the full model object is saved, as the metrics' loader expects.
-    With a `teacher` (any module of logits; not in the reference) the student learns from its args.distill_topk largest logits of each
+    With a `teacher` (any module of logits, put on `device` and into eval mode; not in the reference) the student learns from its args.distill_topk largest logits of each
     sample and the labels (distillation_loss, temperature args.distill_t, weights args.distill_soft and args.distill_hard)."""
     print('\n\nTraining CIFAR-10 Classifier\n\n')
     classifier = Classifier(args=args).to(device) if classifier is None else classifier
@@ -193,6 +193,9 @@ def train_classifier(args, classifier=None, train_dataloader=None, test_dataload
     sched = torch.optim.lr_scheduler.CosineAnnealingLR(optimizer=optim, T_max=args.epochs * len(train_dataloader))
     criterion = nn.CrossEntropyLoss()
     if teacher is not None:
+        learning = {id(t) for t in (*classifier.parameters(), *classifier.buffers())}
+        if any(id(t) in learning for t in (*teacher.parameters(), *teacher.buffers())):
+            raise ValueError("the teacher shares parameters with the classifier that learns from it, which would train the teacher too")
         teacher = teacher.to(device).eval()
 
     def loss_of(outputs, labels, images):

@@ -367,6 +367,31 @@ def test_train_classifier_with_a_teacher(tmp_path, monkeypatch, int8):
     assert not again.int8_fc and "_gmk_fold" not in again.__dict__
 
 
+@pytest.mark.parametrize("shared", ["itself", "inside", "a layer"])
+def test_train_classifier_refuses_a_teacher_that_it_would_train(shared):
+    from models.classifiers import train_classifier
+    student, args = _classifier(2)
+    teacher, _ = _classifier(1)
+    if shared == "a layer":
+        teacher.conv1 = student.conv1
+    teacher = {"itself": student, "inside": torch.nn.Sequential(student), "a layer": teacher}[shared]
+    with pytest.raises(ValueError, match="shares"):
+        train_classifier(args, student, [], [], torch.device("cpu"), teacher=teacher)
+
+
+def test_train_classifier_takes_a_teacher_of_the_same_activation_object(monkeypatch, tmp_path):
+    """Two classifiers of the same arguments share the activation's module, which has no parameters."""
+    from models import classifiers
+    monkeypatch.chdir(tmp_path)
+    os.makedirs("checkpoints")
+    student, args = _classifier(2)
+    args.epochs = 0
+    teacher = classifiers.Classifier(args=args)
+    assert teacher.act is student.act
+    monkeypatch.setattr(torch.optim.lr_scheduler, "CosineAnnealingLR", lambda **k: None)
+    assert classifiers.train_classifier(args, student, [], [], torch.device("cpu"), teacher=teacher) is student
+
+
 def test_flags():
     from arguments import get_args_parser
     a = get_args_parser().parse_args([])
