@@ -89,6 +89,26 @@ def compute_metrics(autoencoder=None, classifier=None, real_images=None, samples
     return fid_classifier, fid_ae, confidence, diversity, inception_score
 
 
+def load_teacher(args, device, unused=None):
+    """The classifier of --teacher_checkpoint, or None.  `unused`: why this run trains no classifier; flags without an effect are named."""
+    flags = [f for f, on in (('--teacher_checkpoint', args.teacher_checkpoint is not None), ('--teacher_int8', args.teacher_int8)) if on]
+    if unused is None and args.teacher_checkpoint is None:
+        unused = 'there is no --teacher_checkpoint'
+    if unused is not None:
+        if flags:
+            print(f'\n\n{" ".join(flags)} ignored: {unused}')
+        return None
+    from models.classifiers import Classifier
+    teacher = torch.load(args.teacher_checkpoint, map_location=device, weights_only=False)
+    if isinstance(teacher, dict):
+        raise NotImplementedError('\n\nteacher checkpoint must be a full saved model, not a state_dict\n\n')
+    if args.teacher_int8 and not isinstance(teacher, Classifier):
+        raise NotImplementedError(f'\n\n--teacher_int8: a {type(teacher).__name__} has no 8-bit layers, a Classifier has\n\n')
+    if isinstance(teacher, Classifier):
+        teacher.int8_fc = args.teacher_int8
+    return teacher
+
+
 def main(args):
     for dir_name in ['checkpoints', 'data', 'plots', 'logs']:
         make_folder(dir_name)
@@ -148,22 +168,18 @@ def main(args):
         from models.classifiers import evaluate_classifier, train_classifier
         classifier_checkpoint = args.classifier_checkpoint or f'checkpoints/cifar_classifier_{args.latent_size}.pth'
         if os.path.isfile(classifier_checkpoint):
+            load_teacher(args, device, unused=f'the classifier is loaded from {classifier_checkpoint}')
             classifier = torch.load(classifier_checkpoint, weights_only=False)
             test_acc = evaluate_classifier(classifier, test_dataloader=test_dataloader, device=device)
             print(f'\n\nCIFAR-10 Test Accuracy {test_acc:.2f}')
         else:
             print(f'\n\nClassifier checkpoint is not found at {classifier_checkpoint}')
-            teacher = None
-            if args.teacher_checkpoint is not None:
-                teacher = torch.load(args.teacher_checkpoint, map_location=device, weights_only=False)
-                if isinstance(teacher, dict):
-                    raise NotImplementedError('\n\nteacher checkpoint must be a full saved model, not a state_dict\n\n')
-                teacher.int8_fc = args.teacher_int8
             classifier = train_classifier(args, classifier=None, train_dataloader=train_dataloader,
-                                          test_dataloader=test_dataloader, device=device, teacher=teacher)
+                                          test_dataloader=test_dataloader, device=device, teacher=load_teacher(args, device))
         if isinstance(plain_ae, dict) or isinstance(classifier, dict):
             raise NotImplementedError('\n\nmodel checkpoint must be a full saved model, not a state_dict\n\n')
     else:
+        load_teacher(args, device, unused='only a --variational run trains a classifier')
         model_type = 'plain-ae'
 
     if args.checkpoint is not None:

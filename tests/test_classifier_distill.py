@@ -398,3 +398,62 @@ def test_flags():
     assert a.teacher_checkpoint is None and not a.teacher_int8 and (a.distill_topk, a.distill_t, a.distill_soft, a.distill_hard) == (3, 4.0, 0.9, 0.1)
     a = get_args_parser().parse_args("--teacher_checkpoint t.pth --teacher_int8 --distill_topk 5 --distill_t 2".split())
     assert a.teacher_checkpoint == "t.pth" and a.teacher_int8 and a.distill_topk == 5 and a.distill_t == 2.0
+
+
+@pytest.mark.parametrize("case", ["plain", "loaded", "trained", "int8 alone", "no flags"])
+def test_main_says_which_teacher_flags_do_nothing(monkeypatch, tmp_path, capsys, case):
+    """main up to the optimizer, with made-up data and models: a teacher is used where a classifier is trained, and named as ignored else."""
+    import main as drv
+    from arguments import get_args_parser
+    from models import classifiers
+
+    class Stop(Exception):
+        pass
+
+    def stop(*a, **k):
+        raise Stop
+
+    monkeypatch.chdir(tmp_path)
+    loader = [(torch.zeros(300, 3, 32, 32), torch.zeros(300))]
+    teacher, _ = _classifier(1)
+    torch.save(teacher, "t.pth")
+    torch.save(torch.nn.Identity(), "ae.pth")
+    torch.save(torch.nn.Identity(), "c.pth")
+    seen = []
+    monkeypatch.setattr(drv, "init_from_env", lambda: (0, 0, 1))
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(drv, "get_cifar", lambda **k: (loader, loader))
+    monkeypatch.setattr(drv, "Autoencoder", lambda **k: types.SimpleNamespace(to=lambda d: torch.nn.Identity()))
+    monkeypatch.setattr(drv, "FusedAdamW", stop)
+    monkeypatch.setattr(classifiers, "evaluate_classifier", lambda *a, **k: 0.0)
+    monkeypatch.setattr(classifiers, "train_classifier", lambda *a, **k: seen.append(k["teacher"]) or torch.nn.Identity())
+    real = torch.load
+    monkeypatch.setattr(torch, "load", lambda f, map_location=None, **k: real(f, map_location="cpu", **k))
+    flags = {"plain": "--teacher_checkpoint t.pth --teacher_int8", "loaded": "--variational --classifier_checkpoint c.pth --teacher_checkpoint t.pth",
+             "trained": "--variational --teacher_checkpoint t.pth --teacher_int8", "int8 alone": "--variational --teacher_int8", "no flags": "--variational"}[case]
+    args = get_args_parser().parse_args(flags.split() + ["--ae_checkpoint", "ae.pth", "--latent_size", "64"])
+    with pytest.raises(Stop):
+        drv.main(args)
+    said = [line for line in capsys.readouterr().out.splitlines() if "ignored" in line]
+    want = {"plain": ["--teacher_checkpoint --teacher_int8 ignored: only a --variational run trains a classifier"],
+            "loaded": ["--teacher_checkpoint ignored: the classifier is loaded from c.pth"], "int8 alone": ["--teacher_int8 ignored: there is no --teacher_checkpoint"]}
+    assert said == want.get(case, [])
+    assert len(seen) == (case in ("trained", "int8 alone", "no flags"))
+    if case == "trained":
+        assert isinstance(seen[0], classifiers.Classifier) and seen[0].int8_fc
+    elif seen:
+        assert seen == [None]
+
+
+def test_teacher_int8_needs_a_classifier(tmp_path):
+    """--teacher_int8 on a model without 8-bit layers would change nothing."""
+    import main as drv
+    torch.save(torch.nn.Linear(3, 2), tmp_path / "t.pth")
+    args = types.SimpleNamespace(teacher_checkpoint=str(tmp_path / "t.pth"), teacher_int8=True)
+    with pytest.raises(NotImplementedError, match="Linear"):
+        drv.load_teacher(args, "cpu")
+    args.teacher_int8 = False
+    assert not hasattr(drv.load_teacher(args, "cpu"), "int8_fc")
+    torch.save(torch.nn.Linear(3, 2).state_dict(), tmp_path / "t.pth")
+    with pytest.raises(NotImplementedError, match="state_dict"):
+        drv.load_teacher(args, "cpu")
