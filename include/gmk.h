@@ -354,7 +354,7 @@ int gmk_linear_i8_fwd(const void* x, int xtype, const signed char* wq, const flo
 
 /* gmk_topk_rows: the k largest of each row of x (n,C): value (n,k) in x's type, index (n,k) int32, in falling order, equal
  *   values by rising index.  -0 equals 0; a NaN ranks above every number; masked classes (-inf, the type's lowest) are ordinary
- *   values.  1 <= k <= min(C, GMK_TOPK_MAX), C < 2^31.  ws >= gmk_topk_rows_workspace_bytes(n, C, k) bytes (0: NULL is fine). */
+ *   values.  1 <= k <= min(C, GMK_TOPK_MAX), C < 2^31 - 1.  ws >= gmk_topk_rows_workspace_bytes(n, C, k) bytes (0: NULL is fine). */
 #define GMK_TOPK_MAX 256
 size_t gmk_topk_rows_workspace_bytes(int64_t n, int64_t C, int k);
 int gmk_topk_rows(const void* x, int xtype, void* value, int* index, int64_t n, int64_t C, int k, void* ws, size_t ws_bytes,
@@ -369,7 +369,7 @@ int gmk_topk_rows(const void* x, int xtype, void* value, int* index, int64_t n, 
  *   (say -100) or labels == NULL: no hard part.  A row with neither part gives loss 0 and gradient 0 whatever its logits hold, and so does one
  *   whose logits are all -inf.  The same class may be
  *   listed more than once.  The soft loss is a difference of sums in 32 bits, known to about soft T^2 2^-20: at temperatures far above the
- *   logits' differences it loses its digits (the gradient does not).  z and dz share ztype, t has ttype.  1 <= k <= GMK_DISTILL_MAX_K, C < 2^31, T between 2^-60 and 2^60.
+ *   logits' differences it loses its digits (the gradient does not).  z and dz share ztype, t has ttype.  1 <= k <= GMK_DISTILL_MAX_K, C < 2^31 - 1, T between 2^-60 and 2^60.
  * gmk_distill_fwd: loss (n) fp32 and stats (n,3) fp32 (the row's maximum and its two sums of exponentials) for the backward pass.
  * gmk_distill_bwd: dz (n,C) = grad[row] * d loss / d z, grad (n) fp32; everything else as in the forward call.  Rows with grad 0 give
  *   0 (nothing of them is read).

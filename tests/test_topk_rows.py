@@ -190,6 +190,15 @@ def test_topk_rows_refusals():
         ops.topk_rows(torch.zeros(2, 5), 2)
 
 
+def test_widest_rows():
+    """2^31 - 2 classes are the most that the header allows, of a top-k and of a distillation (then the missing tensors are what is refused)."""
+    from gmk import lib
+    h = lib()
+    for C, code in (((1 << 31) - 2, -5), ((1 << 31) - 1, -6)):
+        assert h.gmk_topk_rows(None, 0, None, None, 2, C, 5, None, 0, None) == code
+        assert h.gmk_distill_fwd_bwd(None, 0, None, 0, None, None, None, None, None, 2, C, 5, 1.0, 1.0, 0.0, 1.0, None, 0, None) == code
+
+
 @gpu
 def test_topk_rows_refuses_wrong_tensors():
     from gmk import ops
