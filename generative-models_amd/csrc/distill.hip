@@ -12,10 +12,10 @@
 // again (distill_grad_kernel, which is the backward pass too).  The gradient of the listed classes is written over what the dense pass
 // wrote, by the workgroup that wrote it.
 //
-// Measured: 4096x32768 bf16 with labels 125 us, 4.3 TB/s in and out; without them, one exponential less for each logit and for each
-// gradient, 104.5 us and 5.1 TB/s (a copy 5.1 to 5.5): bound by the vector units, then by memory.  1001x10007 fp32 19 us, as loss and
+// Measured: 4096x32768 bf16 with labels 125 to 128 us, 4.2 TB/s in and out; without them, one exponential less for each logit and for each
+// gradient, 106 us and 5.1 TB/s (a copy 5.1 to 5.5): bound by the vector units, then by memory.  1001x10007 fp32 19 us, as loss and
 // backward pass 12 + 18.  256x10 5.1 us, a launch and the
-// latency of its chain of loads and reductions; 9x200003 fp16 10.9 us, two launches.
+// latency of its chain of loads and reductions; 9x200003 fp16 11.1 us, two launches.
 #include "rows.h"
 #include "plan.h"
 
@@ -178,9 +178,9 @@ __device__ __forceinline__ float distill_most(const gmk_u32x4& v, float mx) {
 }
 
 // Elements [e, C) of a row from a piece's values, as far as there are any.  `stream`: whole pieces go past the caches, where the logits stay.
-// For the backward pass and rows in parts always (with the loss before it 4096x32768 bf16 193 us, else 207; 8000x8001 fp16 91.4, else 99.8;
-// 400x200003 fp16 in parts 100, else 113); for a row in registers, where the logits have no more use, if rows are whole lines of 128 bytes
-// (4096x32768 bf16 125, else 132; 8000x8001 fp16 would take 67, else 61.5).
+// For the backward pass and rows in parts always (with the loss before it 4096x32768 bf16 188 us, else 201; 8000x8001 fp16 93.2, else 99.8;
+// 400x200003 fp16 in parts 101, else 113.5); for a row in registers, where the logits have no more use, if rows are whole lines of 128 bytes
+// (4096x32768 bf16 128, else 135; 8000x8001 fp16 would take 67, else 62).
 template <class T>
 __device__ __forceinline__ void distill_put(T* dzr, int64_t e, int64_t C, const float* o, bool stream) {
   constexpr int VEC = gmk_elem<T>::VEC;
@@ -390,8 +390,8 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(const T* __restrict__ 
 static int64_t distill_parts(int64_t C, int vec) { return (C + DISTILL_NT * DISTILL_KEEP * vec - 1) / (DISTILL_NT * DISTILL_KEEP * vec); }
 
 // Rows in parts: those that no workgroup's registers hold (8 pieces for each of 1024 threads), and, for the loss alone, many that only a
-// workgroup of 1024 threads would: 2048x65536 bf16 76 us in parts, whole rows 107.  With the gradient whole rows win, as they are read
-// once: 511 rows of 49000 32.8 us, 512 in parts 40.0.
+// workgroup of 1024 threads would: 2048x65536 bf16 55 us in parts, whole rows 94; 512x49000 17.7 (20.1; the same with 511 rows, which are
+// taken whole).  With the gradient whole rows win, as they are read once: 512x49000 37.2 us, in parts it would take 40.6.
 static bool distill_in_parts(int mode, int64_t n, int64_t C, int vec) {
   const int64_t pieces = (C + vec - 1) / vec;
   return pieces > 8192 || (mode == 0 && n >= 512 && pieces > 4096);
@@ -443,8 +443,9 @@ static int distill_launch(const void* z, int ztype, const DistillArgs& a, const 
       return GMK_OK;
     };
     const int64_t pieces = (a.C + VEC - 1) / VEC;
-    // As few pieces a thread as hold the row (one that no thread has costs what the others do: 4096x20000 bf16 73 us with 5 of 512 threads,
-    // 106 with 8), and as few threads, so that several workgroups of a unit are at different steps.
+    // As few pieces a thread as hold the row (one that no thread has costs what the others do: 4096x20000 bf16 with labels 81 us with 10 of
+    // 256 threads, 118 with 6 of 512 and 129 with 8; 2048x36000 136 with 6 of 1024, 155 with 8), and as few threads, so that several workgroups of a
+    // unit are at different steps (5 of 512 threads would take 86; without labels 71, 10 of 256 75.5).
     if (pieces <= 64 * 1) return go(distill_row_kernel<T, 64, 1, MODE>, 64);
     if (pieces <= 64 * 2) return go(distill_row_kernel<T, 64, 2, MODE>, 64);
     if (pieces <= 64 * 4) return go(distill_row_kernel<T, 64, 4, MODE>, 64);

@@ -35,8 +35,8 @@ __device__ __forceinline__ void i8_put4(const float4& z, T* p, int have) {   // 
   }
 }
 
-// All 4, past the caches, where the operands' tiles stay instead: 8192x4096x16384 446 us (455), 1053x432x29312 33.5 (36.4).  Only where
-// rows are whole lines of 128 bytes: parts of a line that the caches do not join cost 2204x256x29857 81.8 us (43.0).
+// All 4, past the caches, where the operands' tiles stay instead: 1053x432x29312 33.7 us (through them 35.8), 8192x4096x16384 451 to 457 (454
+// to 459).  Only where rows are whole lines of 128 bytes: parts of a line that the caches do not join cost 2204x256x29857 84.7 us (45.2).
 template <class T>
 __device__ __forceinline__ void i8_stream4(const float4& z, T* p) {
   typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -56,10 +56,10 @@ __device__ __forceinline__ void i8_stream4(const float4& z, T* p) {
 // that is permuted: a row's lanes still read its BK bytes in one go.
 // Rows behind the last one and pieces behind K are past the buffer's end for the load, which makes them zeros.
 //
-// Measured, bf16 out: 8192x8192x8192 409 to 420 us, 2620 to 2690 TOP/s (a copy-free loop of the instruction reaches 4000 to 4350);
-// 8192x4096x16384 446 us, with the quantiser before it too (its q is still in the caches).  The matrix cores are busy in 59 % (K = 4096) to
+// Measured, bf16 out: 8192x8192x8192 409 to 422 us, 2600 to 2690 TOP/s (a copy-free loop of the instruction reaches 4000 to 4350);
+// 8192x4096x16384 450 to 457 us, with the quantiser before it 437 to 448 (its q is still in the caches).  The matrix cores are busy in 59 % (K = 4096) to
 // 69 % (K = 8192) of the cycles, at the 1.9 GHz that the card holds under this load; LDS has no bank conflict.  What is left is the end of a
-// tile, when all units write their 128 KB at once: 8192x1024x16384 takes 155 us of which the products are 90.
+// tile, when all units write their 128 KB at once: 8192x1024x16384 takes 154 us of which the products are 90.
 #define I8_BK 128
 __device__ __forceinline__ int i8_place(int row, int piece) { return piece ^ (row & 7); }
 
@@ -87,6 +87,7 @@ struct I8Stage {
   }
   // Load i of the chunk at column k into LDS, `lds` the byte address of this wave's first 64 pieces.  In asm, as the compiler would
   // wait for every load that is out before it reads LDS at all; a load to LDS has no result register, and the loop below counts it.
+  // m0 is a reserved register, which no clobber list may name: the compiler keeps nothing in it and sets it where it needs it itself.
   __device__ __forceinline__ void load(int i, unsigned lds, int first, int k, int K) const {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"((int)lds + i * NTHR * 16), "v"(first + i * STEP * K), "s"(rsrc),
                  "s"(k) : "memory");
@@ -342,11 +343,12 @@ static int gemm_i8_tile_launch(const signed char* xq, const float* xscale, const
 // A workgroup makes NT * 16 columns times 16 rows of y; its waves take turns along K, 64 bytes of each row at a time straight from
 // memory into the instruction's registers, U steps in flight, and their sums meet in LDS.  Rows behind the last one are read from the
 // last one and never stored; behind K the weight's piece is zero.
-// Bound by the weight's bytes: 1x4096x32768 bf16 30.1 us, 4.5 TB/s with the start of the launch, 28.1 from 8-bit rows.
+// Bound by the weight's bytes: 1x4096x32768 bf16 30.5 us, 4.4 TB/s with the start of the launch.
 // X is the rows' type: 8-bit values with xscale, or, for at most I8_FUSED_ROWS rows of floating numbers, x itself, which every workgroup
 // then quantises into its LDS while its first weights are on their way: one launch instead of two.
 #define I8_FUSED_ROWS 4
-#define I8_FUSED_BYTES 16384   // of quantised rows in LDS: 1x4096 30.0 us (two launches 32.0), 4x4096 10.2 (11.7), but 3x8192 22.1 (20.0)
+#define I8_FUSED_BYTES 16384   // of quantised rows in LDS: 1x4096x32768 30.5 us (two launches 41.4), 1x4096x8192 10.4 (13.3), 4x4096x32768 38.5 (41.8),
+                               // 4x4096x4096 10.4 (10.0), but 3x8192x8192 would take 21.9 (19.5)
 template <class T, class X, int NT, int WAVES, int U>
 __global__ __launch_bounds__(64 * WAVES) void gemm_i8_rows_kernel(const X* __restrict__ x, const float* __restrict__ xscale,
                                                                   const signed char* __restrict__ wq, const float* __restrict__ wscale,
@@ -484,14 +486,15 @@ static int gemm_i8_check(int M, int K, int N, int ytype, int act) {
 
 // Which kernel: by the tiles that a shape has, as all that counts is how many of the 256 compute units work and how often each
 // begins anew.  Times in us of the kernel alone on an MI355X (M x K x N, bf16 out):
-//   16x16 with its waves along K: few tiles.  256x4096x256 6.0 (32x32 tiles 9.5), 1x8192x8192 13.9 (15.6), but 64x4096x4096 17.0 (9.6)
-//   32x16 the same way: up to 8 rows, any number of columns.  1x4096x32768 28.1 (64x32 tiles 29.2), but 24 rows 56.8 (29.8)
-//   32x32 tiles: 24x8192x8192 15.6 (64x64 20.4), 64x4096x4096 9.6 (12.2); 24x4096x32768 has twice as many as run at once: 34.0 (29.8)
-//   64x32 tiles: up to 32 rows.  32x4096x32768 30.0 (64x64 31.2), but 64 rows 39.1 (31.9)
+//   16x16 with its waves along K: few tiles.  256x4096x256 6.0 (32x32 tiles 9.3), 1x8192x8192 14.9 (32x16 18.5), but 64x4096x4096 17.6 (9.6)
+//   32x16 the same way: up to 8 rows, any number of columns, which is the form that quantises up to 4 rows by itself (1x4096x32768 bf16 30.5).
+//   From 8-bit rows 64x32 tiles would be faster at these: 1x4096x32768 37.6 (29.3), 8 rows 39.5 (29.4); 24 rows 60.6 (29.9)
+//   32x32 tiles: 24x8192x8192 15.6 (64x64 19.9), 64x4096x4096 9.6 (12.0); 24x4096x32768 has twice as many as run at once: 34.6 (29.9)
+//   64x32 tiles: up to 32 rows.  32x4096x32768 30.1 (64x64 31.3), but 64 rows 39.5 (32.1)
 //   beyond that, the least estimate of rounds * (start and end of a tile + 128-byte chunks of K * time of one), its constants
-//   measured with a unit full of that kernel: 64x64 512x4096x4096 16.3 (128x128 19.3), 128x128 with 8 waves 1024x4096x4096 22.0 (28.4, two
-//   workgroups of 4 waves 26.7), 128 columns by 192 rows 700x2048x7000 16.9 (19.4, 128x128 with 8 waves 22.7), 128x128 with 4 waves
-//   2048x4096x4096 35.0 (40.3, 256x256 45.3), 256x256 4096x4096x4096 54 (64.5)
+//   measured with a unit full of that kernel: 64x64 512x4096x4096 16.2 (128x128 19.4), 128x128 with 8 waves 1024x4096x4096 21.8 (29.0, two
+//   workgroups of 4 waves 25.9), 128 columns by 192 rows 700x2048x7000 16.9 (21.9, 128x128 with 8 waves 22.6), 1500x4096x4096 28.1 (30.6, 37.0),
+//   128x128 with 4 waves 2048x4096x4096 34.6 (40.6, 256x256 43.2), 256x256 4096x4096x4096 55.7 (67.3)
 static int gemm_i8_launch(const signed char* xq, const float* xscale, const signed char* wq, const float* wscale,
                           const float* bias, void* y, int ytype, int M, int K, int N, int act, gmk_stream_t stream) {
   const int cus = i8_cus();
@@ -570,7 +573,7 @@ extern "C" int gmk_linear_i8_fwd(const void* x, int xtype, const signed char* wq
   signed char* q = (signed char*)ws;
   float* s = (float*)(q + linear_i8_q_bytes(M, K));
   // What the product reads again and again, q and the weight, is kept in the last cache (256 MB) by letting x pass it by, once the three
-  // are about half of it: 8192x4096x16384 bf16 451 us (474), 4096x4096x16384 236 (250), but 8192x2048x8192 145 (143).
+  // are about half of it: 8192x4096x16384 bf16 442 to 448 us (468 to 472), 4096x4096x16384 229 (246), but 8192x2048x8192 142.6 (137.5).
   const bool once = (int64_t)M * K * gmk_dtype_size(xtype) + (int64_t)(M + (int64_t)N) * Kp > 100 << 20;
   const int e = gmk_quantize_rows_launch(x, xtype, q, s, M, K, Kp, once, stream);
   if (e != GMK_OK) return e;

@@ -47,9 +47,9 @@ __global__ __launch_bounds__(NT * ROWS) void quantize_rows_kernel(const T* __res
 }
 
 // 1024 threads a row where there are too few rows to fill the card and a row has work for them; a wave a row where rows are short
-// (8192x512 bf16: 6.2 us, with 256 threads 10.1); else 256 threads (8192x2048 fp32: 17.4 us, a wave a row 28.0).  Bound by memory with many
-// rows (8192x4096 bf16: 20.9 us, 4.8 TB/s in and out), by latency with few (256x4096 fp32: 3.8 us, an empty launch 2.6).
-// `once`: x is read past the caches, for the sake of what the caller needs in them afterwards (8192x4096 bf16 alone 24.0 us).
+// (8192x512 bf16: 5.7 us, with 256 threads 10.1); else 256 threads (8192x2048 fp32: 17.6 us, a wave a row 20.6).  Bound by memory with many
+// rows (8192x4096 bf16: 21.0 us, 4.8 TB/s in and out), by latency with few (256x4096 fp32: 3.8 us, with 256 threads a row 4.3, an empty launch 2.6).
+// `once`: x is read past the caches, for the sake of what the caller needs in them afterwards.
 int gmk_quantize_rows_launch(const void* x, int xtype, signed char* q, float* scale, int64_t M, int K, int ldq, bool once,
                              gmk_stream_t stream) {
   return gmk_with_dtype(xtype, [&](auto t) -> int {

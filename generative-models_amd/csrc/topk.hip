@@ -13,7 +13,14 @@
 //
 // Measured: 2048x65536 bf16, k = 32 54.4 us, 4.9 TB/s of the rows' bytes, which is what a maximum over them reads at; 256x1000 fp32, k = 10
 // 4.7 us and 5x150001 fp32, k = 50 11.6 us, the latency of one and of two launches' chains of loads, search and counting.  What
-// is read again grows with k: 512x200000 fp16 40.4 us with k = 10 (5.1 TB/s), 59.6 with k = 128.
+// is read again grows with k: 512x200000 fp16 40.4 us with k = 10 (5.1 TB/s), 59.7 with k = 128.
+//
+// What defeats it: a row or part whose k-th largest thread's maximum is a value that most of its elements have, as the mask's where fewer than
+// k threads hold a class that is not masked.  Every element is then collected, they do not fit, and the search by bits takes five passes in
+// which they all count in one bin.  5x150001 fp32, k = 50: 11.5 us, with the last tenth masked, which fills whole parts, 53, with all but the
+// first 40 classes masked 73 (-inf) or 103 (the lowest value), with equal values 91.  In whole rows a masked tenth or half costs nothing, but
+// with all but the first 40 classes masked, which few threads hold, 2048x65536 bf16, k = 32 takes 1184 us for 54.5, with equal values 1978;
+// 300x60000 fp32, k = 50 499 and 522 for 17.6.  Up to 1024 elements do fit: 256x1000 fp32, k = 10 with equal values 41.5 for 4.7.
 #include "rows.h"
 #include "plan.h"
 
@@ -39,7 +46,7 @@ __device__ __forceinline__ unsigned topk_index(u64 pair) { return 0xFFFFFFFFu - 
 #define TOPK_WAVE 4096       // elements of a row that one wave takes at most
 #define TOPK_PART 4096       // elements of a part that one round of loads of fp32 takes
 #define TOPK_PAIRS 4096      // pairs that a merge holds in LDS at most
-#define TOPK_BLOCKS 512      // workgroups that are worth having, a row has no more parts: 300x60000 fp32, k = 50 17.7 us (with 1024 22.1)
+#define TOPK_BLOCKS 512      // workgroups that are worth having, a row has no more parts: 300x60000 fp32, k = 50 17.6 us (with 1024 22.2)
 
 template <int NT>
 struct TopkShared {
@@ -137,7 +144,7 @@ __device__ __forceinline__ void topk_row(const T* __restrict__ x, int64_t C, uns
   constexpr int64_t LOAD = (int64_t)NT * VEC, GROUP = LOAD * TOPK_LOADS;   // elements of one load of all threads; of one round of loads
   const int tid = threadIdx.x, lane = tid & 63;
   // Rounds of loads, of the row and of a segment; pieces of a segment.  A segment is a single load where there are at most two rounds:
-  // 4000x10000 bf16, k = 100 32.7 us, with whole rounds 37.3.
+  // 4000x10000 bf16, k = 100 33.0 us, with whole rounds 37.3.
   static_assert(TOPK_SEGS == 2 * TOPK_LOADS, "segments of up to two rounds");
   const int64_t groups = (C + GROUP - 1) / GROUP, per_seg = (groups + TOPK_SEGS - 1) / TOPK_SEGS;
   const unsigned pieces = groups <= 2 ? 1u : (unsigned)per_seg * TOPK_LOADS;
@@ -412,8 +419,8 @@ extern "C" int gmk_topk_rows(const void* x, int xtype, void* value, int* index, 
     const T* xt = (const T*)x;
     hipStream_t st = (hipStream_t)stream;
     // One maximum a thread where that makes at least twice k of them, else four.  A wave a row for rows of a few pieces a thread, of more
-    // where the card is full of rows: 8192x1000 fp32 13.0 us, 256 threads 22.7; 4096x4096 bf16, k = 64 16.6 (24.3), but 1024x4000 fp32 12.9
-    // (9.7) and 256x1000 fp32 5.2 (4.7).
+    // where the card is full of rows: 8192x1000 fp32, k = 10 13.0 us, 256 threads 22.7; 4096x4096 bf16, k = 64 16.8 (24.3), but 1024x4000 fp32,
+    // k = 10 7.9 (7.3) and 256x1000 5.2 (4.7).
     const bool many = k <= TOPK_NT / 2 && len >= (int64_t)2 * k * gmk_elem<T>::VEC;
     if (parts == 1) {
       auto go = [&](auto kernel, int nt) -> int {
